@@ -181,6 +181,54 @@ MB_API int mb_gather(mb_ctx* ctx, int32_t layer, int32_t stream, int32_t positio
 MB_API int mb_ring_write(mb_ctx* ctx, int32_t layer, int32_t stream, int32_t first_position, int32_t count,
                          const void* k, const void* v, void* cuda_stream);
 
+/* ---------------------------------------------------------------------------
+ * Searching over continuations.  No counterpart in the reference, which decodes
+ * one token per step and picks greedily: verifying a tree of drafted tokens in
+ * one pass over the rings (mb_tree_attend, mb_tree_commit), and keeping several
+ * hypotheses of an utterance (mb_beam_select below, mb_ring_reorder).
+ *
+ * A tree hangs on a stream whose next position is `positions[i]` (base): node t
+ * has parents[t] = -1 (it follows the ring's last position), an earlier node
+ * u < t, or -2 (absent, to pad trees to one size).  A node with d proper
+ * ancestors stands at position base + d.  1 <= nodes <= 64.  All base + d must be
+ * < max_position, and < capacity on a non-wrapping ring.  An item all of whose
+ * nodes are absent is skipped, whatever its stream and position.  parents:
+ * device int32 [n][nodes].
+ * ------------------------------------------------------------------------- */
+
+/* Attention of n trees over one layer of the rings, which stay as they are: node
+ * t's query attends the slots with 0 <= slot_pos < base and base + d - slot_pos <
+ * capacity, and the nodes on its path (itself included, the last `capacity` of
+ * them), with K after RoPE and V rounded to the storage type -- what
+ * mb_append_attend gives for t when the nodes of its path are appended one after
+ * another.  qkv: device f32 [n][nodes][3*heads*64] (read-only); out: device f32
+ * [n][nodes][heads*64], rows of absent nodes and of rejected items left as they
+ * were.  Live K and V must be finite for finite results; what dead slots and
+ * nodes off the path hold does not matter.  A stream may appear in several items
+ * (the rings are only read). */
+MB_API int mb_tree_attend(mb_ctx* ctx, int32_t layer, int32_t n, int32_t nodes, const int32_t* streams,
+                          const int32_t* positions, const int32_t* parents, const float* qkv, float* out,
+                          void* cuda_stream);
+
+/* Append the accepted path of n trees to the rings of layers [layer, layer +
+ * layers): the nodes on the path to leaves[i] (device int32 [n]; -1: nothing is
+ * accepted) at positions base, base + 1, .., as mb_rope_append would.
+ * qkv: device f32 [layers][n][nodes][3*heads*64], the rows mb_tree_attend took in
+ * each layer; next_positions: device int32 [n] or NULL, base + the path's length
+ * (not written for a rejected item; must not overlap positions). */
+MB_API int mb_tree_commit(mb_ctx* ctx, int32_t layer, int32_t layers, int32_t n, int32_t nodes,
+                          const int32_t* streams, const int32_t* positions, const int32_t* parents,
+                          const int32_t* leaves, const float* qkv, int32_t* next_positions, void* cuda_stream);
+
+/* Permute the rings of `groups` groups of `beams` (1..16) streams, in place and in
+ * every layer: stream streams[g][k] takes the live slots and slot positions that
+ * stream streams[g][parents[g][k]] had before the call; -1 leaves it as it is.
+ * streams, parents: device int32 [groups][beams], a stream at most once per call
+ * (a repeat within a group is rejected, one across groups races).  What a slot
+ * that is empty in the source held in the destination is left there, empty. */
+MB_API int mb_ring_reorder(mb_ctx* ctx, int32_t groups, int32_t beams, const int32_t* streams,
+                           const int32_t* parents, void* cuda_stream);
+
 /* Wait for `cuda_stream` and report device-side rejections (then clear them). */
 MB_API int mb_sync(mb_ctx* ctx, void* cuda_stream);
 
@@ -334,6 +382,37 @@ MB_API int mb_local_head_frame_host(mb_local_head* head, int32_t n, const int32_
  * 2048. */
 MB_API int mb_argmax_penalty(int32_t n, int32_t codes, const float* logits, uint32_t* seen, float penalty,
                              int32_t* tokens, void* cuda_stream);
+
+/* One step of beam search over groups of `beams` (1..16) hypotheses, on the
+ * current device.  With x the logits of a row -- a code whose bit is set in the
+ * row's seen mask first becomes x / penalty (x >= 0) or x * penalty (x < 0), as in
+ * mb_argmax_penalty -- the candidates of beam b are
+ *     (b, j) with value scores[b] + x_j - log(sum_i exp(x_i)),   j in [0, codes)
+ * or, when finished[b] is set, (b, end_id) alone with value scores[b].  A value
+ * that is not finite as fp32 is no candidate, so a beam of score -inf, a code
+ * masked by -inf, a row masked altogether, and a row holding NaN or +inf propose
+ * nothing.  The group's `beams` best candidates, by value and then by lowest
+ * b * codes + j, become
+ *     parents[k] = b, tokens[k] = j, scores_out[k] = value,
+ *     finished_out[k] = finished[b] or j == end_id,
+ *     seen[k] = seen[b], with bit j set unless beam b was finished;
+ * without enough candidates the rest get parents = tokens = -1, scores_out = -inf
+ * and keep their own finished flag and seen mask.  Values are ordered as computed
+ * in 64 bits.
+ *   logits    [groups][beams] rows of `codes` values of `dtype` (mb_dtype),
+ *             row_stride elements apart; only element-aligned
+ *   scores    f32 [groups][beams]; scores_out may be the same array
+ *   finished, finished_out   int32 [groups][beams], both or neither NULL; may be
+ *             the same array; with them end_id must be given
+ *   end_id    a code, or -1
+ *   seen      [groups][beams][codes / 32], updated in place, or NULL (penalty is
+ *             then not used); codes must be a multiple of 32
+ *   parents, tokens   int32 [groups][beams] out
+ * 1 <= codes <= 2^24.  Async on cuda_stream. */
+MB_API int mb_beam_select(int32_t groups, int32_t beams, int32_t codes, int32_t dtype, const void* logits,
+                          int64_t row_stride, const float* scores, float* scores_out, const int32_t* finished,
+                          int32_t* finished_out, int32_t end_id, uint32_t* seen, float penalty, int32_t* parents,
+                          int32_t* tokens, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------
  * No-allocation entry point.  No counterpart in the reference: the reference

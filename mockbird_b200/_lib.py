@@ -105,6 +105,11 @@ SIGNATURES = {
     "mb_decoder_destroy": (ctypes.c_int, [_P]),
     "mb_decoder_step": (ctypes.c_int, [_P, _I, _P, _P, _P, _P]),
     "mb_decoder_step_host": (ctypes.c_int, [_P, _I, _P, _P, _P, _P]),
+    "mb_tree_attend": (ctypes.c_int, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "mb_tree_commit": (ctypes.c_int, [_P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
+    "mb_ring_reorder": (ctypes.c_int, [_P, _I, _I, _P, _P, _P]),
+    "mb_beam_select": (ctypes.c_int, [_I, _I, _I, _I, _P, ctypes.c_int64, _P, _P, _P, _P, _I, _P, ctypes.c_float, _P,
+                                      _P, _P]),
     "mb_set_wait_limit": (ctypes.c_int, [_P, ctypes.c_int64]),
     "mb_local_head_weight_count": (ctypes.c_size_t, [_P, ctypes.POINTER(MbLocalConfig)]),
     "mb_local_head_create": (ctypes.c_int, [_P, ctypes.POINTER(MbLocalConfig), _P, ctypes.c_size_t,

@@ -19,8 +19,8 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libmockbird_kv.so")
 
 SOURCES = ["mb_api.cu", "mb_decode.cu", "mb_decode_persist.cu", "mb_prefill.cu", "mb_prefill_tc.cu", "mb_gemm.cu",
-           "mb_decoder.cu", "mb_local.cu", "mb_noalloc.cu"]
-HEADERS = ["mb_internal.cuh", "mb_ptx.cuh", "mb_decoder.cuh", "mb_gemm.cuh"]
+           "mb_decoder.cu", "mb_local.cu", "mb_noalloc.cu", "mb_tree.cu", "mb_beam.cu"]
+HEADERS = ["mb_internal.cuh", "mb_ptx.cuh", "mb_decoder.cuh", "mb_gemm.cuh", "mb_tree.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 LINK = ["-Xlinker", "-rpath=/usr/local/cuda/lib64"]

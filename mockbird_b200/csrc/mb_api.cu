@@ -64,6 +64,11 @@ int check_batch(mb_ctx* c, int n) {
     return MB_OK;
 }
 
+int check_nodes(mb_ctx* c, int nodes) {
+    if (nodes < 1 || nodes > 64) return fail(c, MB_ERR_ARG, "node count %d out of range [1, 64]", nodes);
+    return MB_OK;
+}
+
 // Host-side checks of one position (decode.ts:719-724 for the non-wrapping ring).
 int check_position(mb_ctx* c, int pos) {
     if (pos < 0 || pos >= c->cfg.max_position)
@@ -343,9 +348,12 @@ int mb::report_bits(mb_ctx* c, int32_t bits) {
     CK(cudaMemset(c->d_err, 0, sizeof(int32_t)), "clear device status");
     if (bits & DERR_TIMEOUT)
         return fail(c, MB_ERR_TIMEOUT, "a bounded device-side wait gave up (bits 0x%x)", bits);
-    return fail(c, MB_ERR_DEVICE, "a kernel rejected an item:%s%s%s", (bits & DERR_STREAM) ? " stream out of range" : "",
+    return fail(c, MB_ERR_DEVICE, "a kernel rejected an item:%s%s%s%s%s",
+                (bits & DERR_STREAM) ? " stream out of range" : "",
                 (bits & DERR_POSITION) ? " position out of range" : "",
-                (bits & DERR_CAPACITY) ? " position beyond a non-wrapping ring" : "");
+                (bits & DERR_CAPACITY) ? " position beyond a non-wrapping ring" : "",
+                (bits & DERR_TREE) ? " tree parent or leaf out of range" : "",
+                (bits & DERR_PARENT) ? " beam parent out of range" : "");
 }
 
 extern "C" {
@@ -567,6 +575,62 @@ MB_API int mb_ring_write(mb_ctx* c, int32_t layer, int32_t stream, int32_t first
     CK(launch_ring_write(c->cfg.dtype, ring_view(c, layer), stream, first_position, count, k, v,
                          static_cast<cudaStream_t>(cuda_stream)),
        "ring_write launch");
+    return MB_OK;
+}
+
+MB_API int mb_tree_attend(mb_ctx* c, int32_t layer, int32_t n, int32_t nodes, const int32_t* streams,
+                          const int32_t* positions, const int32_t* parents, const float* qkv, float* out,
+                          void* cuda_stream) {
+    if (!c) return MB_ERR_ARG;
+    int rc;
+    if ((rc = check_layer(c, layer)) || (rc = check_batch(c, n)) || (rc = check_nodes(c, nodes))) return rc;
+    if (n == 0) return MB_OK;
+    if (!streams || !positions || !parents || !qkv || !out || !aligned(qkv, 16) || !aligned(out, 16) ||
+        !aligned(streams, 4) || !aligned(positions, 4) || !aligned(parents, 4))
+        return fail(c, MB_ERR_ARG, "null or misaligned device pointer");
+    DeviceGuard g(c->cfg.device);
+    CK(launch_tree_attend(c->cfg.dtype, ring_view(c, layer), n, nodes, streams, positions, parents, qkv, out,
+                          static_cast<cudaStream_t>(cuda_stream)),
+       "tree_attend launch");
+    return MB_OK;
+}
+
+MB_API int mb_tree_commit(mb_ctx* c, int32_t layer, int32_t layers, int32_t n, int32_t nodes, const int32_t* streams,
+                          const int32_t* positions, const int32_t* parents, const int32_t* leaves, const float* qkv,
+                          int32_t* next_positions, void* cuda_stream) {
+    if (!c) return MB_ERR_ARG;
+    int rc;
+    if ((rc = check_layer(c, layer)) || (rc = check_batch(c, n)) || (rc = check_nodes(c, nodes))) return rc;
+    if (layers <= 0 || layers > c->cfg.layers - layer)
+        return fail(c, MB_ERR_LAYER, "%d layers from layer %d exceed the context's %d", layers, layer, c->cfg.layers);
+    if (n == 0) return MB_OK;
+    if (!streams || !positions || !parents || !leaves || !qkv || !aligned(qkv, 16) || !aligned(streams, 4) ||
+        !aligned(positions, 4) || !aligned(parents, 4) || !aligned(leaves, 4) || !aligned(next_positions, 4))
+        return fail(c, MB_ERR_ARG, "null or misaligned device pointer");
+    // (several blocks read an item's position while one writes the next)
+    if (next_positions && next_positions < positions + n && positions < next_positions + n)
+        return fail(c, MB_ERR_ARG, "next_positions overlaps positions");
+    DeviceGuard g(c->cfg.device);
+    CK(launch_tree_commit(c->cfg.dtype, ring_view(c, layer), layers, n, nodes, streams, positions, parents, leaves,
+                          qkv, next_positions, static_cast<cudaStream_t>(cuda_stream)),
+       "tree_commit launch");
+    return MB_OK;
+}
+
+MB_API int mb_ring_reorder(mb_ctx* c, int32_t groups, int32_t beams, const int32_t* streams, const int32_t* parents,
+                           void* cuda_stream) {
+    if (!c) return MB_ERR_ARG;
+    if (beams < 1 || beams > 16) return fail(c, MB_ERR_ARG, "beam count %d out of range [1, 16]", beams);
+    if (groups < 0 || groups > 65535 || (int64_t)groups * beams > c->cfg.streams)
+        return fail(c, MB_ERR_ARG, "%d groups of %d beams exceed the context's %d streams", groups, beams,
+                    c->cfg.streams);
+    if (groups == 0) return MB_OK;
+    if (!streams || !parents || !aligned(streams, 4) || !aligned(parents, 4))
+        return fail(c, MB_ERR_ARG, "null or misaligned device pointer");
+    DeviceGuard g(c->cfg.device);
+    CK(launch_ring_reorder(c->cfg.dtype, ring_view(c, 0), c->cfg.layers, groups, beams, streams, parents,
+                           static_cast<cudaStream_t>(cuda_stream)),
+       "ring_reorder launch");
     return MB_OK;
 }
 

@@ -26,6 +26,8 @@ enum : int32_t {
     DERR_POSITION = 2,
     DERR_CAPACITY = 4,
     DERR_TIMEOUT = 8,
+    DERR_TREE = 16,    // a tree's parent or leaf
+    DERR_PARENT = 32,  // a beam's parent
 };
 
 // Everything a kernel needs to address one layer of the rings.
@@ -149,6 +151,17 @@ cudaError_t launch_gather(int dtype, const RingView& r, int stream, int position
 cudaError_t launch_ring_write(int dtype, const RingView& r, int stream, int first, int count, const void* k,
                               const void* v, cudaStream_t st);
 cudaError_t launch_reset(const mb_ctx* c, int stream, cudaStream_t st);
+
+// Searching over continuations (mb_tree.cu, mb_beam.cu).  r: the layer's rings
+// (launch_tree_commit and launch_ring_reorder cover `layers` layers from it).
+cudaError_t launch_tree_attend(int dtype, const RingView& r, int n, int nodes, const int32_t* streams,
+                               const int32_t* positions, const int32_t* parents, const float* qkv, float* out,
+                               cudaStream_t st);
+cudaError_t launch_tree_commit(int dtype, const RingView& r, int layers, int n, int nodes, const int32_t* streams,
+                               const int32_t* positions, const int32_t* parents, const int32_t* leaves,
+                               const float* qkv, int32_t* next_positions, cudaStream_t st);
+cudaError_t launch_ring_reorder(int dtype, const RingView& r, int layers, int groups, int beams,
+                                const int32_t* streams, const int32_t* parents, cudaStream_t st);
 
 // host-array entry points (mb_api.cu): checks of the items on the host, and the
 // status of the device rejection bits a call read back (cleared on the device;

@@ -18,6 +18,8 @@ decode.ts:719-724):
     PrefillRunner.run's rope/scores/softmax/     KvRing.prefill
       apply dispatches (prefill.ts:424-462)
     PrefillRunner.readLayerCache (:644-664)      KvRing.read_layer_cache
+    (none: one token per step, greedy)           KvRing.tree_attend, KvRing.tree_commit,
+                                                 KvRing.reorder, beam_select
     PrefillRunner.poisonKv (:610-620)            KvRing.poison_kv
     WgpuTtsEngineImpl.reset / resetRings         KvRing.reset
       (gpu.ts:237-242, codec.ts:279-282)
@@ -58,6 +60,14 @@ def _ptr(t) -> ctypes.c_void_p:
 # The raw handle of a device's current CUDA stream: torch's C accessor where
 # this torch has it (no Stream object per call), else the public API.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _used_on(stream, t: torch.Tensor) -> None:
+    """Tell the caching allocator that `t`, made on the current stream, is used on
+    `stream`: its memory is then not handed out again before that use is over."""
+    if stream is not None and t.is_cuda:
+        t.record_stream(stream if isinstance(stream, torch.cuda.Stream)
+                        else torch.cuda.ExternalStream(int(stream), device=t.device))
 
 
 _TORCH_DTYPE = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
@@ -254,6 +264,85 @@ class KvRing:
         self._check(self.lib.mb_prefill(self.ctx, layer, n, _ptr(s), rows, _ptr(q), _ptr(self._dev(out)),
                                         self._stream(stream)))
         return out
+
+    # ------------------------------------------------------------ searching over continuations
+    def tree_attend(self, layer: int, streams, positions, parents, qkv: torch.Tensor,
+                    out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """Attention of a tree of drafted tokens per item over one layer's rings, which stay as they are.
+
+        positions [n]: each stream's next position.  parents [n][nodes] (nodes <= 64): an earlier
+        node, -1 (follows the ring's last position) or -2 (absent: its row of `out` is not written).
+        qkv [n][nodes][3*H*64] -> context [n][nodes][H*64]; node t's row is what append_attend gives
+        for t when the nodes of its path are appended one after another."""
+        n, nodes = self._tree_shape(qkv, 3)
+        s, p = self._id_array("streams", streams, (n,), stream), self._id_array("positions", positions, (n,), stream)
+        tree = self._id_array("parents", parents, (n, nodes), stream)
+        if out is None:
+            out = torch.empty(n, nodes, self.hidden, dtype=torch.float32, device=self.device)
+            _used_on(stream, out)
+        else:
+            self._array("out", out, (n, nodes, self.hidden), torch.float32)
+        self._check(self.lib.mb_tree_attend(self.ctx, layer, n, nodes, s.data_ptr(), p.data_ptr(), tree.data_ptr(),
+                                            qkv.data_ptr(), out.data_ptr(), self._stream(stream)))
+        return out
+
+    def tree_commit(self, layer: int, streams, positions, parents, leaves, qkv: torch.Tensor,
+                    next_positions: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """Append each tree's accepted path, the nodes up to leaves[i] (-1: none), to the rings of
+        qkv.shape[0] layers from `layer`, as rope_split_ring would one after another.
+
+        qkv [layers][n][nodes][3*H*64]: the rows tree_attend took in each layer.  Returns
+        next_positions [n] int32, each position moved behind its path (not `positions` itself)."""
+        n, nodes = self._tree_shape(qkv, 4)
+        s, p = self._id_array("streams", streams, (n,), stream), self._id_array("positions", positions, (n,), stream)
+        tree, leaf = self._id_array("parents", parents, (n, nodes), stream), self._id_array("leaves", leaves, (n,), stream)
+        if next_positions is None:
+            next_positions = torch.empty(n, dtype=torch.int32, device=self.device)
+            _used_on(stream, next_positions)
+        else:
+            self._array("next_positions", next_positions, (n,), torch.int32)
+        self._check(self.lib.mb_tree_commit(self.ctx, layer, qkv.shape[0], n, nodes, s.data_ptr(), p.data_ptr(),
+                                            tree.data_ptr(), leaf.data_ptr(), qkv.data_ptr(),
+                                            next_positions.data_ptr(), self._stream(stream)))
+        return next_positions
+
+    def reorder(self, streams, parents, stream=None) -> None:
+        """Permute the rings of beam groups in place, all layers: stream streams[g][k] takes the
+        state that stream streams[g][parents[g][k]] had before the call; -1 leaves it as it is.
+
+        streams, parents: [groups][beams] (beams <= 16), e.g. beam_select's parents."""
+        s = self._id_array("streams", streams, None, stream)
+        if s.dim() != 2:
+            raise ValueError(f"streams must be [groups][beams] (got {tuple(s.shape)})")
+        up = self._id_array("parents", parents, tuple(s.shape), stream)
+        self._check(self.lib.mb_ring_reorder(self.ctx, s.shape[0], s.shape[1], s.data_ptr(), up.data_ptr(),
+                                             self._stream(stream)))
+
+    def _array(self, name: str, t, shape, dtype) -> torch.Tensor:
+        """A contiguous tensor of `shape` and `dtype` on the ring's device."""
+        if not (isinstance(t, torch.Tensor) and t.device == self.device and t.dtype is dtype and t.is_contiguous()):
+            raise TypeError(f"{name} must be a contiguous {dtype} tensor on {self.device}")
+        if shape is not None and t.shape != shape:
+            raise ValueError(f"{name} must be of shape {list(shape)} (got {list(t.shape)})")
+        return t
+
+    def _id_array(self, name: str, values, shape, stream) -> torch.Tensor:
+        """An int32 array of `shape`: a device tensor as it is, or host values copied to the device."""
+        if isinstance(values, torch.Tensor) and values.is_cuda:
+            return self._array(name, values, shape, torch.int32)
+        t = torch.as_tensor(np.ascontiguousarray(values, np.int32), device=self.device)
+        if shape is not None and t.shape != shape:
+            raise ValueError(f"{name} must be of shape {list(shape)} (got {list(t.shape)})")
+        _used_on(stream, t)
+        return t
+
+    def _tree_shape(self, qkv, dims: int) -> tuple[int, int]:
+        """(items, nodes) of a tree's qkv rows, [..][n][nodes][3*H*64]."""
+        self._array("qkv", qkv, None, torch.float32)
+        if qkv.dim() != dims or qkv.shape[-1] != 3 * self.hidden:
+            raise ValueError(f"qkv must have {dims} dimensions, the last of 3*heads*64 = {3 * self.hidden} "
+                             f"(got {list(qkv.shape)})")
+        return qkv.shape[-3], qkv.shape[-2]
 
     # ------------------------------------------------------------ cache access
     def gather(self, layer: int, stream_id: int, position: int, stream=None):
@@ -479,3 +568,54 @@ def argmax_penalty(logits: torch.Tensor, seen: torch.Tensor, penalty: float, str
     if rc:
         raise MockbirdError(rc, "mb_argmax_penalty: bad arguments or launch failure")
     return out
+
+
+_DTYPE_CODE = {torch.float32: _lib.MB_F32, torch.bfloat16: _lib.MB_BF16, torch.float16: _lib.MB_F16}
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None = None, end_id: int = -1,
+                seen: torch.Tensor | None = None, penalty: float = 1.0, stream=None):
+    """One beam-search step on the device: the best `beams` continuations of each group.
+
+    logits [groups][beams][codes] fp32, bf16 or fp16, rows contiguous and evenly spaced (a padded
+    vocabulary is read in place); scores [groups][beams] fp32, each hypothesis' log probability
+    (-inf: no hypothesis); finished [groups][beams] int32 with end_id, the code that ends one: a
+    finished beam goes on as it is.  seen [groups][beams][codes/32] int32: codes already emitted,
+    penalised as argmax_penalty does; updated in place, each row following its new hypothesis.
+
+    Returns (parents, tokens, scores, finished), each [groups][beams], new tensors; finished is None
+    when not given.  Without enough candidates parent and token are -1 and the score is -inf."""
+    lib = _lib.load()
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dtype in _DTYPE_CODE and logits.dim() == 3):
+        raise TypeError("logits must be a 3-D CUDA tensor of float32, bfloat16 or float16")
+    groups, beams, codes = logits.shape
+    row = logits.stride(1) if beams > 1 else logits.stride(0) if groups > 1 else codes
+    if (codes > 1 and logits.stride(2) != 1) or (beams > 1 and groups > 1 and logits.stride(0) != beams * row):
+        raise TypeError("logits' rows must be contiguous and evenly spaced")
+    dev = logits.device
+    for name, t, dtype, shape in (("scores", scores, torch.float32, (groups, beams)),
+                                  ("finished", finished, torch.int32, (groups, beams)),
+                                  ("seen", seen, torch.int32, (groups, beams, codes // 32))):
+        if t is None and name != "scores":
+            continue
+        if not (isinstance(t, torch.Tensor) and t.device == dev and t.dtype is dtype and t.is_contiguous()
+                and t.shape == shape):
+            raise TypeError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {dev}")
+    new = torch.empty(3 if finished is None else 4, groups, beams, dtype=torch.int32, device=dev)
+    _used_on(stream, new)
+    parents, tokens, out = new[0], new[1], new[2].view(torch.float32)
+    done = None if finished is None else new[3]
+    if stream is None:
+        stream = _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+    elif isinstance(stream, torch.cuda.Stream):
+        stream = stream.cuda_stream
+    with torch.cuda.device(dev):
+        rc = lib.mb_beam_select(groups, beams, codes, _DTYPE_CODE[logits.dtype], logits.data_ptr(), row,
+                                scores.data_ptr(), out.data_ptr(), None if finished is None else finished.data_ptr(),
+                                None if done is None else done.data_ptr(), end_id,
+                                None if seen is None else seen.data_ptr(), penalty, parents.data_ptr(),
+                                tokens.data_ptr(), int(stream))
+    if rc:
+        raise MockbirdError(rc, f"mb_beam_select: bad arguments or launch failure (groups={groups} beams={beams} "
+                                f"codes={codes} end_id={end_id} penalty={penalty})")
+    return parents, tokens, out, done
