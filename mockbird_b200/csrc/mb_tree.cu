@@ -11,6 +11,13 @@
 //   nodes of its path are appended one after another.
 #include "mb_tree.cuh"
 
+#include <cooperative_groups.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "mb_ptx.cuh"
+
 namespace mb {
 
 namespace {
@@ -24,91 +31,645 @@ __device__ __forceinline__ T from_f(float v) {
     return static_cast<T>(v);
 }
 
-// One warp per node, one slot per lane: every lane keeps the running maximum,
-// sum and context of its slots, and the warp joins them at the end.
+// ---------------------------------------------------------------- matrix instructions and copies
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 16-byte asynchronous copy to shared memory; `live` false fills with zeros and reads nothing
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+
+// d[16 x 8] += a b with fp32 accumulation: bf16 or f16 operands 16 deep, tf32 operands 8 deep
 template <typename T>
-__global__ void __launch_bounds__(128) tree_attend_kernel(RingView r, int nodes, const int32_t* __restrict__ streams,
-                                                          const int32_t* __restrict__ positions,
-                                                          const int32_t* __restrict__ parents,
-                                                          const float* __restrict__ qkv, float* __restrict__ out) {
-    __shared__ TreeShape sh;
-    __shared__ __align__(16) float sq[4][HD];
-    const int H = r.heads, C = r.capacity, item = blockIdx.x / H, h = blockIdx.x % H;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) tree_shape(sh, parents + (size_t)item * nodes, nodes, lane);
+__device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 4)
+        asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+            "%2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    else if constexpr (std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+            "%2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+            "%2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// ---------------------------------------------------------------- operands in parts
+//
+// The context is fp32 accurate: what is narrower than fp32 on the tensor cores is
+// the operand, and an operand is held as a sum of parts whose products are added.
+//   bf16 rings  K, V are bf16 as they are; q and the weights in 3 bf16 parts (8 bits each: all 24)
+//   f16 rings   K, V are f16 as they are; q and the weights in 2 f16 parts (22 bits), scaled by a power of
+//               two so that the second part stays clear of f16's smallest numbers
+//   fp32 rings  every operand in 2 tf32 parts (11 + 11 bits), three products (lo lo, 2^-22 of hi hi, is left out)
+template <typename T>
+struct Parts {  // bf16
+    static constexpr int N = 3;
+    static constexpr float SHIFT = 0.f;  // log2 of the weights' scale
+};
+template <>
+struct Parts<__half> {
+    static constexpr int N = 2;
+    static constexpr float SHIFT = 14.f;  // weights in [0, 2^14]: the second part is exact to 2^-38 of the largest
+};
+template <>
+struct Parts<float> {
+    static constexpr int N = 2;
+    static constexpr float SHIFT = 0.f;
+};
+
+constexpr uint32_t TF32_MASK = 0xFFFFE000u;
+
+__device__ __forceinline__ void tf32_parts(float x, uint32_t& hi, uint32_t& lo) {
+    hi = __float_as_uint(x) & TF32_MASK;
+    // the rest is exact and rounded to its 11 leading bits (to nearest, ties away)
+    lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & TF32_MASK;
+}
+
+// p[i]: the packed 16-bit parts of (x, y), largest first
+template <typename T>
+__device__ __forceinline__ void pair_parts(float x, float y, uint32_t (&p)[Parts<T>::N]) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x, y);
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+        p[0] = *reinterpret_cast<const uint32_t*>(&h);
+        p[1] = *reinterpret_cast<const uint32_t*>(&l);
+    } else {  // the upper halves of the fp32 words: truncation, so the rests are exact
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+            p[i] = __byte_perm(u, v, 0x7632);
+            x -= __uint_as_float(u & 0xFFFF0000u);
+            y -= __uint_as_float(v & 0xFFFF0000u);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- tree attention
+//
+// A block takes 16 * MT nodes (the rows of MT matrix tiles) of one item and head,
+// over every `splits`-th group of four tiles of slots; the blocks of the other
+// splits form its cluster.  Each warp runs on its own: it copies its tiles of TS
+// slots (4 KB of K, 4 KB of V) into its own two stages, and keeps the running
+// maximum, sum and context of its rows in registers, so nothing in the loop waits
+// for another warp.  The tree's own K and V follow the ring's tiles as tiles of the
+// same layout, built from the qkv rows.  At the end the warps join through shared
+// memory, then the blocks of the cluster through distributed shared memory: no
+// scratch in device memory, so calls share nothing.
+template <typename T>
+struct Tile {
+    static constexpr int SLOTS = sizeof(T) == 4 ? 16 : 32;
+    static constexpr int ROW16 = sizeof(T) * HD / 16;  // 16-byte pieces per row
+    static constexpr int BYTES = SLOTS * HD * sizeof(T);
+    // Piece c of row j lies at piece c ^ swizzle: the eight rows (ldmatrix) or the
+    // rows and pieces (fp32 reads) that one access phase touches fall in different
+    // banks.
+    __device__ static int kswz(int j) { return sizeof(T) == 4 ? (j & 1) * 4 : j & 7; }
+    __device__ static int vswz(int j) { return sizeof(T) == 4 ? ((j >> 1) & 1) + ((j >> 2) & 1) * 4 : j & 7; }
+};
+constexpr int WARPS = 4, STAGES = 2;
+
+template <typename T, int MT>
+struct alignas(16) TreeSmem {
+    unsigned char stage[WARPS][STAGES][2 * Tile<T>::BYTES];  // K, then V
+    // q as matrix operands: [part][tile][step][lane]
+    uint4 q[Parts<T>::N][MT][sizeof(T) == 4 ? 8 : 4][32];
+    float m[WARPS][16 * MT], l[WARPS][16 * MT];  // [0]: the block's after the join
+    float scale[16 * MT];                        // of a score in units of log2
+    unsigned int qmax[16 * MT];
+    TreeShape shape;
+};
+
+template <typename T, int MT>
+__global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int nodes, int qtiles, int splits,
+                                                                 const int32_t* __restrict__ streams,
+                                                                 const int32_t* __restrict__ positions,
+                                                                 const int32_t* __restrict__ parents,
+                                                                 const float* __restrict__ qkv,
+                                                                 float* __restrict__ out) {
+    using Tl = Tile<T>;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int TS = Tl::SLOTS, NT = TS / 8, ROWS = 16 * MT, QSTEPS = F32 ? 8 : 4, NP = Parts<T>::N;
+    extern __shared__ unsigned char smem_raw[];
+    TreeSmem<T, MT>& sm = *reinterpret_cast<TreeSmem<T, MT>*>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, quad = lane & 3;
+    const int H = r.heads, C = r.capacity;
+    const int rank = blockIdx.x % splits, qt = (blockIdx.x / splits) % qtiles;
+    const int h = (blockIdx.x / splits / qtiles) % H, item = blockIdx.x / splits / qtiles / H;
+
+    if (warp == 0) tree_shape(sm.shape, parents + (size_t)item * nodes, nodes, lane);
+    if (tid < ROWS) sm.qmax[tid] = 0u;
     __syncthreads();
-    if (!sh.bad && sh.max_depth < 0) return;
+    const TreeShape& sh = sm.shape;
+    const int max_depth = sh.max_depth;
+    if (!sh.bad && max_depth < 0) return;
     const int s = streams[item], base = positions[item];
     if (const int why = tree_reject(r, sh, s, base)) {
-        if (threadIdx.x == 0 && h == 0) atomicOr(r.err, why);
+        if (blockIdx.x % (splits * qtiles * H) == 0 && tid == 0) atomicOr(r.err, why);
         return;
     }
     const T* K = reinterpret_cast<const T*>(r.kv) + (((size_t)s * 2 + 0) * H + h) * (size_t)C * HD;
     const T* V = K + (size_t)H * C * HD;
     const int32_t* sp = r.slot_pos + (size_t)s * C;
-    const size_t row = (size_t)3 * H * HD;
-    const float* rows = qkv + (size_t)item * nodes * row + h * HD;
+    const size_t row_f = (size_t)3 * H * HD;
+    const float* rows = qkv + (size_t)item * nodes * row_f + h * HD;
+    const int t0 = qt * ROWS;
     const int window = min(base, C);
-    for (int t = warp; t < nodes; t += 4) {
-        const unsigned long long path = sh.path[t];
-        if (!path) continue;
-        const int depth = __popcll(path) - 1, pos = base + depth;
-        __syncwarp();
-        {
-            const float2 q = reinterpret_cast<const float2*>(rows + t * row)[lane];
-            reinterpret_cast<float2*>(sq[warp])[lane] = rope_pair(q, r.rope[(size_t)pos * 32 + lane]);
-        }
-        __syncwarp();
-        float m = -INFINITY, l = 0.f, o[HD];
+    const int ring_tiles = (window + TS - 1) / TS, tiles = ring_tiles + (nodes + TS - 1) / TS;
+    const int step = splits * WARPS;
+
+    // a ring slot is seen by nodes of depth <= seen_to (-1: by none)
+    auto load_seen = [&](int tile) {
+        const int j = tile * TS + (lane & (TS - 1));
+        if (tile >= ring_tiles || j >= window) return -1;
+        const int p = sp[j];
+        return p >= 0 && p < base ? C - 1 - (base - p) : -1;
+    };
+    unsigned char* const stages = sm.stage[warp][0];
+    // Starts the copies of a ring tile, or builds a tile of the tree's own K and V.
+    // Returns, for a tree tile, the nodes whose V is not finite.
+    auto fill = [&](int tile, int st, int seen_to) -> uint32_t {
+        unsigned char* kd = stages + st * 2 * Tl::BYTES;
+        if (tile < ring_tiles) {
+            const uint32_t live = __ballot_sync(0xffffffffu, seen_to >= 0);
+            const uint32_t ks = smem_u32(kd), vs = ks + Tl::BYTES;
+            const char* kg = reinterpret_cast<const char*>(K) + (size_t)tile * Tl::BYTES;
+            const char* vg = reinterpret_cast<const char*>(V) + (size_t)tile * Tl::BYTES;
 #pragma unroll
-        for (int d = 0; d < HD; d++) o[d] = 0.f;
-        for (int j = lane; j < window + nodes; j += 32) {
-            float k[HD], v[HD];
-            if (j < window) {
-                const int p = sp[j];
-                if (p < 0 || p >= base || pos - p >= C) continue;
-#pragma unroll
-                for (int d = 0; d < HD; d++) k[d] = to_f(K[(size_t)j * HD + d]), v[d] = to_f(V[(size_t)j * HD + d]);
-            } else {
-                const int u = j - window;
-                if (!((path >> u) & 1ull)) continue;
-                const int du = __popcll(sh.path[u]) - 1;
-                if (depth - du >= C) continue;
-                const float2* kr = reinterpret_cast<const float2*>(rows + u * row + (size_t)H * HD);
-                const float* vr = rows + u * row + (size_t)2 * H * HD;
-#pragma unroll
-                for (int d = 0; d < HD / 2; d++) {
-                    const float2 kk = rope_pair(kr[d], r.rope[(size_t)(base + du) * 32 + d]);
-                    k[2 * d] = to_f(from_f<T>(kk.x)), k[2 * d + 1] = to_f(from_f<T>(kk.y));
-                    v[2 * d] = to_f(from_f<T>(vr[2 * d])), v[2 * d + 1] = to_f(from_f<T>(vr[2 * d + 1]));
-                }
+            for (int i = 0; i < TS * Tl::ROW16 / 32; i++) {
+                const int e = i * 32 + lane, j = e / Tl::ROW16, c = e % Tl::ROW16;
+                const bool on = (live >> j) & 1u;
+                const size_t at = on ? (size_t)e * 16 : 0;
+                cp16(ks + (j * Tl::ROW16 + (c ^ Tl::kswz(j))) * 16, kg + at, on);
+                cp16(vs + (j * Tl::ROW16 + (c ^ Tl::vswz(j))) * 16, vg + at, on);
             }
-            float x = 0.f;
-#pragma unroll
-            for (int d = 0; d < HD; d++) x = fmaf(sq[warp][d], k[d], x);
-            x *= SCALE * LOG2E;
-            const float mn = fmaxf(m, x), a = exp2f(m - mn), p = exp2f(x - mn);
-            m = mn;
-            l = l * a + p;
-#pragma unroll
-            for (int d = 0; d < HD; d++) o[d] = o[d] * a + p * v[d];
+            return 0u;
         }
-        const float M = [&] {
-            float g = m;
-            for (int i = 16; i > 0; i >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, i));
-            return g;
-        }();
-        const float a = m == -INFINITY ? 0.f : exp2f(m - M);  // a lane without a visible slot
-        float L = l * a;
-        for (int i = 16; i > 0; i >>= 1) L += __shfl_xor_sync(0xffffffffu, L, i);
-        float* dst = out + ((size_t)item * nodes + t) * H * HD + h * HD;
+        // one row at a time: lane i ropes the pair of dims (2 i, 2 i + 1)
+        uint32_t bad = 0u;
+        const int u0 = (tile - ring_tiles) * TS;
+        constexpr int PP = 16 / (2 * sizeof(T));  // pairs per 16-byte piece
+#pragma unroll 4
+        for (int j = 0; j < TS; j++) {
+            const int u = u0 + j;
+            float2 k = make_float2(0.f, 0.f), v = k;
+            const unsigned long long path = u < nodes ? sh.path[u] : 0ull;
+            if (path) {
+                const float* src = rows + u * row_f;
+                const int pos = base + __popcll(path) - 1;
+                k = rope_pair(reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane], r.rope[(size_t)pos * 32 + lane]);
+                v = reinterpret_cast<const float2*>(src + (size_t)2 * H * HD)[lane];
+            }
+            T kk[2] = {from_f<T>(k.x), from_f<T>(k.y)}, vv[2] = {from_f<T>(v.x), from_f<T>(v.y)};
+            const bool odd = !isfinite(to_f(vv[0])) || !isfinite(to_f(vv[1]));
+            if (__any_sync(0xffffffffu, odd)) bad |= 1u << j;
+            unsigned char* ka = kd + (j * Tl::ROW16 + ((lane / PP) ^ Tl::kswz(j))) * 16 + (lane % PP) * 2 * sizeof(T);
+            unsigned char* va =
+                kd + Tl::BYTES + (j * Tl::ROW16 + ((lane / PP) ^ Tl::vswz(j))) * 16 + (lane % PP) * 2 * sizeof(T);
+            if constexpr (F32) {
+                *reinterpret_cast<float2*>(ka) = make_float2(kk[0], kk[1]);
+                *reinterpret_cast<float2*>(va) = make_float2(vv[0], vv[1]);
+            } else {
+                reinterpret_cast<T*>(ka)[0] = kk[0], reinterpret_cast<T*>(ka)[1] = kk[1];
+                reinterpret_cast<T*>(va)[0] = vv[0], reinterpret_cast<T*>(va)[1] = vv[1];
+            }
+        }
+        return bad;
+    };
+
+    int tile = rank * WARPS + warp;
+    int seen_cur = load_seen(tile), seen_next = load_seen(tile + step);
+    uint32_t bad_cur = 0u;
+    if (tile < tiles) bad_cur = fill(tile, 0, seen_cur);
+    cp_commit();
+
+    // The block's rows of q: roped, scaled (f16), split, in the order the matrix
+    // instructions take them.
+    {
+        constexpr int FRAGS = MT * QSTEPS * 32 / (32 * WARPS), PAIRS = F32 ? 2 : 4;
+        float2 x[FRAGS][PAIRS];
 #pragma unroll
-        for (int d = 0; d < HD; d++) {
-            float g = o[d] * a;
-            for (int i = 16; i > 0; i >>= 1) g += __shfl_xor_sync(0xffffffffu, g, i);
-            if (lane == (d & 31)) dst[d] = g / L;
+        for (int f = 0; f < FRAGS; f++) {
+            const int ks = (f * WARPS + warp) % QSTEPS, mt = (f * WARPS + warp) / QSTEPS;
+#pragma unroll
+            for (int i = 0; i < PAIRS; i++) {
+                // i: row grp / grp + 8, then (16-bit) the pair 8 dims on
+                const int row = mt * 16 + grp + (i & 1) * 8, t = t0 + row;
+                const int d = F32 ? (ks >> 1) * 16 + quad * 4 + (ks & 1) * 2 : ks * 16 + quad * 2 + (i >> 1) * 8;
+                const unsigned long long path = t < nodes ? sh.path[t] : 0ull;
+                x[f][i] = make_float2(0.f, 0.f);
+                if (path) {
+                    const int pos = base + __popcll(path) - 1;
+                    x[f][i] = rope_pair(*reinterpret_cast<const float2*>(rows + t * row_f + d),
+                                        r.rope[(size_t)pos * 32 + d / 2]);
+                }
+                if constexpr (std::is_same<T, __half>::value)
+                    atomicMax(&sm.qmax[row], __float_as_uint(fmaxf(fabsf(x[f][i].x), fabsf(x[f][i].y))));
+            }
+        }
+        if constexpr (std::is_same<T, __half>::value) __syncthreads();
+        // f16: the row's largest |q| goes to [2^13, 2^14)
+        auto up = [&](int row) {
+            const int e = (int)((sm.qmax[row] >> 23) & 255u) - 127;
+            return e == 128 ? 0 : min(13 - e, 100);
+        };
+        auto pow2 = [](int e) { return __int_as_float((e + 127) << 23); };  // e in [-114, 114]
+        if (tid < ROWS) {
+            float c = SCALE * LOG2E;
+            if constexpr (std::is_same<T, __half>::value) c *= pow2(-up(tid));
+            sm.scale[tid] = c;
+        }
+#pragma unroll
+        for (int f = 0; f < FRAGS; f++) {
+            const int ks = (f * WARPS + warp) % QSTEPS, mt = (f * WARPS + warp) / QSTEPS;
+            if constexpr (F32) {
+                uint4 hi, lo;  // rows (grp, grp + 8) x (even, odd dim)
+                tf32_parts(x[f][0].x, hi.x, lo.x), tf32_parts(x[f][1].x, hi.y, lo.y);
+                tf32_parts(x[f][0].y, hi.z, lo.z), tf32_parts(x[f][1].y, hi.w, lo.w);
+                sm.q[0][mt][ks][lane] = hi;
+                sm.q[1][mt][ks][lane] = lo;
+            } else {
+                uint32_t p[4][NP];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float2 v = x[f][i];
+                    if constexpr (std::is_same<T, __half>::value) {
+                        const float e = pow2(up(mt * 16 + grp + (i & 1) * 8));
+                        v.x *= e, v.y *= e;
+                    }
+                    pair_parts<T>(v.x, v.y, p[i]);
+                }
+#pragma unroll
+                for (int k = 0; k < NP; k++) sm.q[k][mt][ks][lane] = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
+            }
         }
     }
+    __syncthreads();
+
+    float m[MT][2], l[MT][2], o[MT][8][4], sc[MT][2];
+    int depth[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int row = mt * 16 + grp + 8 * e, t = t0 + row;
+            m[mt][e] = -INFINITY, l[mt][e] = 0.f, sc[mt][e] = sm.scale[row];
+            depth[mt][e] = t < nodes ? __popcll(sh.path[t]) - 1 : -1;
+        }
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[mt][i][e] = 0.f;
+
+    for (int st = 0; tile < tiles; tile += step, st ^= 1) {
+        // the next tile's copies, then this one's arrival
+        uint32_t bad_next = 0u;
+        if (tile + step < tiles) bad_next = fill(tile + step, st ^ 1, seen_next);
+        cp_commit();
+        const int seen_after = load_seen(tile + 2 * step);
+        cp_wait<1>();
+        __syncwarp();
+        const unsigned char* kd = stages + st * 2 * Tl::BYTES;
+        const uint32_t ks = smem_u32(kd), vs = ks + Tl::BYTES;
+
+        // scores
+        float x[MT][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[mt][i][e] = 0.f;
+        if constexpr (F32) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {  // 16 dims: two steps of 8, dims 4 quad .. + 3 of them in this lane
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const int row = i * 8 + grp;
+                    const float4 k = *reinterpret_cast<const float4*>(
+                        kd + (row * Tl::ROW16 + ((j * 4 + quad) ^ Tl::kswz(row))) * 16);
+                    uint32_t hi[4], lo[4];
+                    tf32_parts(k.x, hi[0], lo[0]), tf32_parts(k.y, hi[1], lo[1]);
+                    tf32_parts(k.z, hi[2], lo[2]), tf32_parts(k.w, hi[3], lo[3]);
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            const uint4 qh = sm.q[0][mt][2 * j + e][lane], ql = sm.q[1][mt][2 * j + e][lane];
+                            mma<T>(x[mt][i], ql, hi[2 * e], hi[2 * e + 1]);
+                            mma<T>(x[mt][i], qh, lo[2 * e], lo[2 * e + 1]);
+                            mma<T>(x[mt][i], qh, hi[2 * e], hi[2 * e + 1]);
+                        }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {  // 16 dims
+                uint32_t k[NT / 2][4];     // two groups of 8 slots each: dims 0-7, 8-15 of the first, of the second
+#pragma unroll
+                for (int i = 0; i < NT / 2; i++) {
+                    const int row = i * 16 + (lane >> 4) * 8 + (lane & 7), c = j * 2 + ((lane >> 3) & 1);
+                    ldsm4(k[i], ks + (row * Tl::ROW16 + (c ^ Tl::kswz(row))) * 16);
+                }
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        const uint4 q = sm.q[p][mt][j][lane];
+#pragma unroll
+                        for (int i = 0; i < NT; i++) mma<T>(x[mt][i], q, k[i / 2][(i & 1) * 2], k[i / 2][(i & 1) * 2 + 1]);
+                    }
+            }
+        }
+
+        // masks: a column is slot 8 i + 2 quad + (e & 1), a row grp (e < 2) or grp + 8
+        uint32_t bad = 0u;  // rows of V that are not finite and not seen by every node
+        const bool in_ring = tile < ring_tiles;
+        if (!in_ring) {
+            const int u0 = (tile - ring_tiles) * TS;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int t = t0 + mt * 16 + grp + 8 * e;
+                    unsigned long long path = t < nodes ? sh.path[t] : 0ull;
+                    // only the last `capacity` of the path, whose earlier nodes have lower indices
+                    for (int over = __popcll(path) - C; over > 0; over--) path &= path - 1ull;
+                    const uint32_t see = (uint32_t)(path >> u0) >> (2 * quad);
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        if (!((see >> (8 * i)) & 1u)) x[mt][i][2 * e] = -INFINITY;
+                        if (!((see >> (8 * i + 1)) & 1u)) x[mt][i][2 * e + 1] = -INFINITY;
+                    }
+                }
+            bad = bad_cur;
+        } else if (!__all_sync(0xffffffffu, seen_cur >= max_depth)) {
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                const int s0 = __shfl_sync(0xffffffffu, seen_cur, 8 * i + 2 * quad);
+                const int s1 = __shfl_sync(0xffffffffu, seen_cur, 8 * i + 2 * quad + 1);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        if (depth[mt][e] > s0 || s0 < 0) x[mt][i][2 * e] = -INFINITY;
+                        if (depth[mt][e] > s1 || s1 < 0) x[mt][i][2 * e + 1] = -INFINITY;
+                    }
+            }
+            // (dead slots hold zeros; these are the ones that only some nodes see)
+            uint32_t some = __ballot_sync(0xffffffffu, seen_cur >= 0 && seen_cur < max_depth) & (TS == 32 ? ~0u : 0xFFFFu);
+            for (; some; some &= some - 1u) {
+                const int j = __ffs(some) - 1;
+                const T* v = reinterpret_cast<const T*>(kd + Tl::BYTES + j * HD * sizeof(T));
+                if (__any_sync(0xffffffffu, !isfinite(to_f(v[lane])) || !isfinite(to_f(v[lane + 32])))) bad |= 1u << j;
+            }
+        }
+
+        // weights
+        float alpha[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NT; i++) top = fmaxf(top, fmaxf(x[mt][i][2 * e], x[mt][i][2 * e + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float mn = fmaxf(m[mt][e], top * sc[mt][e]);
+                const float use = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
+                alpha[mt][e] = ex2(m[mt][e] - use);
+                m[mt][e] = mn;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int f = 0; f < 2; f++) {
+                        const float p = ex2(fmaf(x[mt][i][2 * e + f], sc[mt][e], Parts<T>::SHIFT - use));
+                        x[mt][i][2 * e + f] = p;
+                        sum += p;
+                    }
+                l[mt][e] = fmaf(l[mt][e], alpha[mt][e], sum);
+            }
+        if (bad) {
+            // Rows of V that are not finite reach only the nodes that see them: added one by one, then set to
+            // zero for the products below (whose weights of the other nodes are zero, and 0 * inf is not).
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[mt][i][e] *= alpha[mt][e >> 1];
+                alpha[mt][0] = alpha[mt][1] = 1.f;
+                for (uint32_t b = bad; b; b &= b - 1u) {
+                    const int j = __ffs(b) - 1;
+                    float p0 = 0.f, p1 = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+                        if (i == (j >> 3)) {
+                            const float a0 = x[mt][i][0], a1 = x[mt][i][1], a2 = x[mt][i][2], a3 = x[mt][i][3];
+                            p0 = (j & 1) ? a1 : a0, p1 = (j & 1) ? a3 : a2;
+                        }
+                    p0 = __shfl_sync(0xffffffffu, p0, (lane & ~3) | ((j & 7) >> 1));
+                    p1 = __shfl_sync(0xffffffffu, p1, (lane & ~3) | ((j & 7) >> 1));
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+#pragma unroll
+                        for (int f = 0; f < 2; f++) {
+                            const int d = F32 ? 16 * quad + 8 * f + i : 8 * i + 2 * quad + f;
+                            const int at = (j * Tl::ROW16 + ((d * (int)sizeof(T) / 16) ^ Tl::vswz(j))) * 16 +
+                                           d * (int)sizeof(T) % 16;
+                            const float v = to_f(*reinterpret_cast<const T*>(kd + Tl::BYTES + at));
+                            if (p0 != 0.f) o[mt][i][f] = fmaf(p0, v, o[mt][i][f]);
+                            if (p1 != 0.f) o[mt][i][2 + f] = fmaf(p1, v, o[mt][i][2 + f]);
+                        }
+                }
+            }
+            __syncwarp();
+            for (uint32_t b = bad; b; b &= b - 1u) {
+                unsigned char* row = stages + st * 2 * Tl::BYTES + Tl::BYTES + (__ffs(b) - 1) * HD * sizeof(T);
+                if (lane < Tl::ROW16) reinterpret_cast<uint4*>(row)[lane] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            __syncwarp();
+        }
+
+        // The context of this tile on its own, then one rounding into the running one: the tensor cores'
+        // accumulation does not round to nearest, so its chains stay a tile long.
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            float ot[8][4];
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) ot[i][e] = 0.f;
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < NT; i++) {  // 8 slots: step depth k = quad is slot 2 quad, quad + 4 slot 2 quad + 1
+                    uint4 ph, pl;
+                    tf32_parts(x[mt][i][0], ph.x, pl.x), tf32_parts(x[mt][i][2], ph.y, pl.y);
+                    tf32_parts(x[mt][i][1], ph.z, pl.z), tf32_parts(x[mt][i][3], ph.w, pl.w);
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {  // dims 8 grp + 4 c .. + 3: one for each of four column groups
+                        const int j0 = i * 8 + 2 * quad, j1 = j0 + 1;
+                        const float4 a = *reinterpret_cast<const float4*>(
+                            kd + Tl::BYTES + (j0 * Tl::ROW16 + ((2 * grp + c) ^ Tl::vswz(j0))) * 16);
+                        const float4 b = *reinterpret_cast<const float4*>(
+                            kd + Tl::BYTES + (j1 * Tl::ROW16 + ((2 * grp + c) ^ Tl::vswz(j1))) * 16);
+                        const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                        for (int f = 0; f < 4; f++) {
+                            uint32_t h0, l0, h1, l1;
+                            tf32_parts(av[f], h0, l0), tf32_parts(bv[f], h1, l1);
+                            mma<T>(ot[4 * c + f], pl, h0, h1);
+                            mma<T>(ot[4 * c + f], ph, l0, l1);
+                            mma<T>(ot[4 * c + f], ph, h0, h1);
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NT / 2; i++) {  // 16 slots
+                    uint32_t pp[4][NP];
+#pragma unroll
+                    for (int f = 0; f < 2; f++) {
+                        pair_parts<T>(x[mt][2 * i + f][0], x[mt][2 * i + f][1], pp[2 * f]);
+                        pair_parts<T>(x[mt][2 * i + f][2], x[mt][2 * i + f][3], pp[2 * f + 1]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {  // 16 dims
+                        uint32_t v[4];
+                        const int row = i * 16 + (lane & 15);
+                        ldsm4t(v, vs + (row * Tl::ROW16 + ((2 * c + (lane >> 4)) ^ Tl::vswz(row))) * 16);
+#pragma unroll
+                        for (int p = NP - 1; p >= 0; p--) {
+                            const uint4 a = make_uint4(pp[0][p], pp[1][p], pp[2][p], pp[3][p]);
+                            mma<T>(ot[2 * c], a, v[0], v[1]);
+                            mma<T>(ot[2 * c + 1], a, v[2], v[3]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[mt][i][e] = fmaf(o[mt][i][e], alpha[mt][e >> 1], ot[i][e]);
+        }
+        __syncwarp();  // before the stage is filled again
+        seen_cur = seen_next, seen_next = seen_after, bad_cur = bad_next;
+    }
+    cp_wait<0>();
+    __syncwarp();
+
+    // Join: each warp's rows to its own stages, then the warps' into the first.
+    float* mine = reinterpret_cast<float*>(sm.stage[warp][0]);
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int row = mt * 16 + grp + 8 * e;
+            float sum = l[mt][e];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (quad == 0) sm.m[warp][row] = m[mt][e], sm.l[warp][row] = sum;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if constexpr (F32) {
+                    mine[row * HD + 16 * quad + i] = o[mt][i][2 * e];
+                    mine[row * HD + 16 * quad + 8 + i] = o[mt][i][2 * e + 1];
+                } else {
+                    *reinterpret_cast<float2*>(mine + row * HD + 8 * i + 2 * quad) =
+                        make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
+                }
+            }
+        }
+    __syncthreads();
+    const size_t out_row = (size_t)H * HD;
+    float* dst = out + ((size_t)item * nodes + t0) * out_row + h * HD;
+    for (int i = tid; i < ROWS * 16; i += 32 * WARPS) {
+        const int row = i >> 4, d = (i & 15) * 4;
+        float top = sm.m[0][row];
+#pragma unroll
+        for (int w = 1; w < WARPS; w++) top = fmaxf(top, sm.m[w][row]);
+        const float use = top == -INFINITY ? 0.f : top;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            const float a = ex2(sm.m[w][row] - use);
+            const float4 v = *reinterpret_cast<const float4*>(sm.stage[w][0] + (row * HD + d) * 4);
+            acc.x = fmaf(a, v.x, acc.x), acc.y = fmaf(a, v.y, acc.y);
+            acc.z = fmaf(a, v.z, acc.z), acc.w = fmaf(a, v.w, acc.w);
+            sum = fmaf(a, sm.l[w][row], sum);
+        }
+        if (splits == 1) {
+            if (t0 + row < nodes && sh.path[t0 + row]) {
+                const float inv = 1.f / sum;
+                *reinterpret_cast<float4*>(dst + row * out_row + d) =
+                    make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            }
+        } else {
+            *reinterpret_cast<float4*>(sm.stage[0][0] + (row * HD + d) * 4) = acc;
+            __syncwarp();  // the row's m and l are read by the 16 lanes of this half-warp before they are replaced
+            if (d == 0) sm.m[0][row] = top, sm.l[0][row] = sum;
+        }
+    }
+    if (splits == 1) return;
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    // rows rank, rank + splits, .. from every block of the cluster
+    for (int i = tid; i < ROWS / splits * 16; i += 32 * WARPS) {
+        const int row = (i >> 4) * splits + rank, d = (i & 15) * 4;
+        float top = -INFINITY;
+        for (int b = 0; b < splits; b++) top = fmaxf(top, *cluster.map_shared_rank(&sm.m[0][row], b));
+        const float use = top == -INFINITY ? 0.f : top;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+        for (int b = 0; b < splits; b++) {
+            const float a = ex2(*cluster.map_shared_rank(&sm.m[0][row], b) - use);
+            const float4 v = *cluster.map_shared_rank(reinterpret_cast<float4*>(sm.stage[0][0] + (row * HD + d) * 4), b);
+            acc.x = fmaf(a, v.x, acc.x), acc.y = fmaf(a, v.y, acc.y);
+            acc.z = fmaf(a, v.z, acc.z), acc.w = fmaf(a, v.w, acc.w);
+            sum = fmaf(a, *cluster.map_shared_rank(&sm.l[0][row], b), sum);
+        }
+        if (t0 + row < nodes && sh.path[t0 + row]) {
+            const float inv = 1.f / sum;
+            *reinterpret_cast<float4*>(dst + row * out_row + d) =
+                make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        }
+    }
+    cluster.sync();  // no block leaves while another reads its shared memory
 }
 
 // grid (node groups, items, layers), heads * 16 threads: each thread ropes and
@@ -170,11 +731,45 @@ __global__ void __launch_bounds__(1024) tree_commit_kernel(RingView r, int n, in
     }
 }
 
+template <typename T, int MT>
+cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* streams, const int32_t* positions,
+                      const int32_t* parents, const float* qkv, float* out, cudaStream_t st) {
+    constexpr int smem = sizeof(TreeSmem<T, MT>);
+    // the opt-in to more than 48 KB of shared memory, once per device
+    static std::atomic<uint64_t> opted{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev > 63 || !(opted.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(tree_attend_kernel<T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        opted.fetch_or(bit, std::memory_order_release);
+    }
+    const int qtiles = (nodes + 16 * MT - 1) / (16 * MT);
+    const int tiles = (r.capacity + Tile<T>::SLOTS - 1) / Tile<T>::SLOTS + (nodes + Tile<T>::SLOTS - 1) / Tile<T>::SLOTS;
+    const int blocks = n * r.heads * qtiles;
+    int splits = 1;
+    while (splits < 8 && blocks * splits < 2 * 148 && splits * WARPS < tiles) splits *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks * splits);
+    cfg.blockDim = dim3(32 * WARPS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)splits, 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = splits > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, tree_attend_kernel<T, MT>, r, nodes, qtiles, splits, streams, positions, parents,
+                              qkv, out);
+}
+
 template <typename T>
 cudaError_t attend_t(const RingView& r, int n, int nodes, const int32_t* streams, const int32_t* positions,
                      const int32_t* parents, const float* qkv, float* out, cudaStream_t st) {
-    tree_attend_kernel<T><<<n * r.heads, 128, 0, st>>>(r, nodes, streams, positions, parents, qkv, out);
-    return cudaGetLastError();
+    return nodes <= 16 ? attend_mt<T, 1>(r, n, nodes, streams, positions, parents, qkv, out, st)
+                       : attend_mt<T, 2>(r, n, nodes, streams, positions, parents, qkv, out, st);
 }
 
 template <typename T>
