@@ -12,6 +12,8 @@
 #include "mb_tree.cuh"
 
 #include <cooperative_groups.h>
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 #include <atomic>
 #include <type_traits>
@@ -37,16 +39,6 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-
-// 16-byte asynchronous copy to shared memory; `live` false fills with zeros and reads nothing
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
@@ -106,17 +98,19 @@ struct Parts<float> {
     static constexpr float SHIFT = 0.f;
 };
 
-constexpr uint32_t TF32_MASK = 0xFFFFE000u;
-
+__device__ __forceinline__ uint32_t to_tf32(float x) {  // to nearest
+    uint32_t y;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ void tf32_parts(float x, uint32_t& hi, uint32_t& lo) {
-    hi = __float_as_uint(x) & TF32_MASK;
-    // the rest is exact and rounded to its 11 leading bits (to nearest, ties away)
-    lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & TF32_MASK;
+    hi = to_tf32(x);
+    lo = to_tf32(x - __uint_as_float(hi));
 }
 
 // p[i]: the packed 16-bit parts of (x, y), largest first
 template <typename T>
-__device__ __forceinline__ void pair_parts(float x, float y, uint32_t (&p)[Parts<T>::N]) {
+__device__ __forceinline__ void pair_parts(float x, float y, uint32_t* p) {
     if constexpr (std::is_same<T, __half>::value) {
         const __half2 h = __floats2half2_rn(x, y);
         const float2 f = __half22float2(h);
@@ -136,108 +130,127 @@ __device__ __forceinline__ void pair_parts(float x, float y, uint32_t (&p)[Parts
 
 // ---------------------------------------------------------------- tree attention
 //
-// A block takes 16 * MT nodes (the rows of MT matrix tiles) of one item and head,
-// over every `splits`-th group of four tiles of slots; the blocks of the other
-// splits form its cluster.  Each warp runs on its own: it copies its tiles of TS
-// slots (4 KB of K, 4 KB of V) into its own two stages, and keeps the running
-// maximum, sum and context of its rows in registers, so nothing in the loop waits
-// for another warp.  The tree's own K and V follow the ring's tiles as tiles of the
-// same layout, built from the qkv rows.  At the end the warps join through shared
-// memory, then the blocks of the cluster through distributed shared memory: no
-// scratch in device memory, so calls share nothing.
+// A block takes NODES nodes of one item and head, over every `splits`-th group of
+// WARPS tiles of slots; the blocks of the other splits form its cluster.  Each warp
+// runs on its own: TMA brings its tiles of SLOTS slots (4 KB of K, 4 KB of V) into
+// its own two stages, and it keeps the running maximum, sum and context of its rows
+// in registers, so nothing in the loop waits for another warp.  The tree's own K
+// and V follow the ring's tiles as tiles of the same layout, built from the qkv
+// rows.  At the end the warps join through shared memory, then the blocks of the
+// cluster through distributed shared memory: no scratch in device memory, so calls
+// share nothing.
+//
+// The rows of a matrix tile are 16 nodes, or (PACK, at most 8 nodes) two parts of
+// the same 8 nodes, whose products the lane that holds both adds up.
+constexpr int WARPS = 4, STAGES = 2;
+#ifndef SPLIT_BELOW
+#define SPLIT_BELOW 296
+#endif
+
 template <typename T>
 struct Tile {
     static constexpr int SLOTS = sizeof(T) == 4 ? 16 : 32;
-    static constexpr int ROW16 = sizeof(T) * HD / 16;  // 16-byte pieces per row
     static constexpr int BYTES = SLOTS * HD * sizeof(T);
-    // Piece c of row j lies at piece c ^ swizzle: the eight rows (ldmatrix) or the
-    // rows and pieces (fp32 reads) that one access phase touches fall in different
-    // banks.
-    __device__ static int kswz(int j) { return sizeof(T) == 4 ? (j & 1) * 4 : j & 7; }
-    __device__ static int vswz(int j) { return sizeof(T) == 4 ? ((j >> 1) & 1) + ((j >> 2) & 1) * 4 : j & 7; }
+    static constexpr int HALF = SLOTS * 128;  // one box: 128 bytes of each row
+    // Where TMA's 128-byte swizzle puts 16-byte piece c of row j: an fp32 row spans
+    // two boxes, and within a box pieces are exchanged by the row's low bits, so
+    // the eight rows that ldmatrix reads at once lie in different banks.
+    __device__ static int at(int j, int c) {
+        return sizeof(T) == 4 ? (c >> 3) * HALF + j * 128 + (((c & 7) ^ (j & 7)) << 4) : j * 128 + ((c ^ (j & 7)) << 4);
+    }
 };
-constexpr int WARPS = 4, STAGES = 2;
 
-template <typename T, int MT>
-struct alignas(16) TreeSmem {
+template <typename T, int MT, bool PACK>
+struct alignas(1024) TreeSmem {
+    static constexpr int NODES = PACK ? 8 : 16 * MT;
+    static constexpr int QSETS = sizeof(T) == 4 ? (PACK ? 1 : 2) : PACK ? (Parts<T>::N + 1) / 2 : Parts<T>::N;
     unsigned char stage[WARPS][STAGES][2 * Tile<T>::BYTES];  // K, then V
-    // q as matrix operands: [part][tile][step][lane]
-    uint4 q[Parts<T>::N][MT][sizeof(T) == 4 ? 8 : 4][32];
-    float m[WARPS][16 * MT], l[WARPS][16 * MT];  // [0]: the block's after the join
-    float scale[16 * MT];                        // of a score in units of log2
-    unsigned int qmax[16 * MT];
+    uint4 q[QSETS][MT][sizeof(T) == 4 ? 8 : 4][32];          // q as matrix operands: [part][tile][step][lane]
+    unsigned long long full[WARPS][STAGES], never;           // copies landed; never signalled (mb_set_wait_limit)
+    float m[WARPS][NODES], l[WARPS][NODES];                  // [0]: the block's after the join
+    float scale[NODES];                                      // of a score in units of log2
+    unsigned int qmax[NODES];
     TreeShape shape;
 };
 
-template <typename T, int MT>
-__global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int nodes, int qtiles, int splits,
-                                                                 const int32_t* __restrict__ streams,
-                                                                 const int32_t* __restrict__ positions,
-                                                                 const int32_t* __restrict__ parents,
-                                                                 const float* __restrict__ qkv,
-                                                                 float* __restrict__ out) {
+template <typename T, int MT, bool PACK>
+__global__ void __launch_bounds__(32 * WARPS)
+    tree_attend_kernel(const __grid_constant__ CUtensorMap map, RingView r, int nodes, int qtiles, int splits,
+                       const int32_t* __restrict__ streams, const int32_t* __restrict__ positions,
+                       const int32_t* __restrict__ parents, const float* __restrict__ qkv, float* __restrict__ out) {
     using Tl = Tile<T>;
-    constexpr bool F32 = sizeof(T) == 4;
-    constexpr int TS = Tl::SLOTS, NT = TS / 8, ROWS = 16 * MT, QSTEPS = F32 ? 8 : 4, NP = Parts<T>::N;
-    extern __shared__ unsigned char smem_raw[];
-    TreeSmem<T, MT>& sm = *reinterpret_cast<TreeSmem<T, MT>*>(smem_raw);
+    using Sm = TreeSmem<T, MT, PACK>;
+    constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value;
+    constexpr int TS = Tl::SLOTS, NT = TS / 8, NODES = Sm::NODES, QSTEPS = F32 ? 8 : 4, NP = Parts<T>::N;
+    constexpr int RH = PACK ? 1 : 2;  // rows of a tile in one lane
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, quad = lane & 3;
     const int H = r.heads, C = r.capacity;
     const int rank = blockIdx.x % splits, qt = (blockIdx.x / splits) % qtiles;
     const int h = (blockIdx.x / splits / qtiles) % H, item = blockIdx.x / splits / qtiles / H;
 
-    if (warp == 0) tree_shape(sm.shape, parents + (size_t)item * nodes, nodes, lane);
-    if (tid < ROWS) sm.qmax[tid] = 0u;
-    __syncthreads();
-    const TreeShape& sh = sm.shape;
-    const int max_depth = sh.max_depth;
-    if (!sh.bad && max_depth < 0) return;
+    // The ring's first tiles are on their way before the tree is looked at.
     const int s = streams[item], base = positions[item];
-    if (const int why = tree_reject(r, sh, s, base)) {
-        if (blockIdx.x % (splits * qtiles * H) == 0 && tid == 0) atomicOr(r.err, why);
-        return;
-    }
-    const T* K = reinterpret_cast<const T*>(r.kv) + (((size_t)s * 2 + 0) * H + h) * (size_t)C * HD;
-    const T* V = K + (size_t)H * C * HD;
-    const int32_t* sp = r.slot_pos + (size_t)s * C;
-    const size_t row_f = (size_t)3 * H * HD;
-    const float* rows = qkv + (size_t)item * nodes * row_f + h * HD;
-    const int t0 = qt * ROWS;
-    const int window = min(base, C);
+    const bool in_range = s >= 0 && s < r.streams && base >= 0;
+    const int window = in_range ? min(base, C) : 0;
     const int ring_tiles = (window + TS - 1) / TS, tiles = ring_tiles + (nodes + TS - 1) / TS;
     const int step = splits * WARPS;
-
-    // a ring slot is seen by nodes of depth <= seen_to (-1: by none)
-    auto load_seen = [&](int tile) {
-        const int j = tile * TS + (lane & (TS - 1));
-        if (tile >= ring_tiles || j >= window) return -1;
-        const int p = sp[j];
-        return p >= 0 && p < base ? C - 1 - (base - p) : -1;
-    };
+    const size_t plane = in_range ? ((size_t)s * 2 * H + h) * C : 0;  // K's rows in the map; V's lie H * C on
+    const int32_t* sp = r.slot_pos + (in_range ? (size_t)s * C : 0);
+    uint64_t* const full = reinterpret_cast<uint64_t*>(sm.full[warp]);
     unsigned char* const stages = sm.stage[warp][0];
-    // Starts the copies of a ring tile, or builds a tile of the tree's own K and V.
-    // Returns, for a tree tile, the nodes whose V is not finite.
-    auto fill = [&](int tile, int st, int seen_to) -> uint32_t {
-        unsigned char* kd = stages + st * 2 * Tl::BYTES;
-        if (tile < ring_tiles) {
-            const uint32_t live = __ballot_sync(0xffffffffu, seen_to >= 0);
-            const uint32_t ks = smem_u32(kd), vs = ks + Tl::BYTES;
-            const char* kg = reinterpret_cast<const char*>(K) + (size_t)tile * Tl::BYTES;
-            const char* vg = reinterpret_cast<const char*>(V) + (size_t)tile * Tl::BYTES;
+    auto fetch = [&](int tile, int st) {
+        if (lane == 0) {
+            unsigned char* kd = stages + st * 2 * Tl::BYTES;
+            const int row = (int)plane + tile * TS;
+            mbar_expect_tx(&full[st], 2 * Tl::BYTES);
 #pragma unroll
-            for (int i = 0; i < TS * Tl::ROW16 / 32; i++) {
-                const int e = i * 32 + lane, j = e / Tl::ROW16, c = e % Tl::ROW16;
-                const bool on = (live >> j) & 1u;
-                const size_t at = on ? (size_t)e * 16 : 0;
-                cp16(ks + (j * Tl::ROW16 + (c ^ Tl::kswz(j))) * 16, kg + at, on);
-                cp16(vs + (j * Tl::ROW16 + (c ^ Tl::vswz(j))) * 16, vg + at, on);
+            for (int c = 0; c < Tl::BYTES / Tl::HALF; c++) {
+                tma_load_2d(kd + c * Tl::HALF, &map, c * 32, row, &full[st]);
+                tma_load_2d(kd + Tl::BYTES + c * Tl::HALF, &map, c * 32, row + H * C, &full[st]);
             }
-            return 0u;
         }
-        // one row at a time: lane i ropes the pair of dims (2 i, 2 i + 1)
-        uint32_t bad = 0u;
-        const int u0 = (tile - ring_tiles) * TS;
+    };
+    auto slot_position = [&](int tile) {
+        const int j = tile * TS + (lane & (TS - 1));
+        return j < window ? sp[j] : -1;
+    };
+    int tile = rank * WARPS + warp;
+    int sp_cur = slot_position(tile), sp_next = slot_position(tile + step);
+    if (lane == 0) {
+        mbar_init(&full[0], 1), mbar_init(&full[1], 1);
+        if (warp == 0) mbar_init(reinterpret_cast<uint64_t*>(&sm.never), 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    if (tile < ring_tiles) fetch(tile, 0);
+    if (tile + step < ring_tiles) fetch(tile + step, 1);
+    if (warp == 0) tree_shape(sm.shape, parents + (size_t)item * nodes, nodes, lane);
+    if (tid < NODES) sm.qmax[tid] = 0u;
+    __syncthreads();
+
+    const TreeShape& sh = sm.shape;
+    const int max_depth = sh.max_depth, t0 = qt * NODES;
+    const bool absent = !sh.bad && max_depth < 0;
+    const int why = absent ? 0 : tree_reject(r, sh, s, base);
+    if (absent || why) {
+        if (why && blockIdx.x % (splits * qtiles * H) == 0 && tid == 0) atomicOr(r.err, why);
+        // no block leaves its shared memory while copies into it are under way
+        if (tile < ring_tiles) mbar_wait(&full[0], 0, WAIT_LIMIT);
+        if (tile + step < ring_tiles) mbar_wait(&full[1], 0, WAIT_LIMIT);
+        return;
+    }
+    const size_t row_f = (size_t)3 * H * HD;
+    const float* rows = qkv + (size_t)item * nodes * row_f + h * HD;
+
+    // Builds a tile of the tree's own K and V, one row at a time: lane i ropes dims
+    // (2 i, 2 i + 1).  Returns the nodes whose V is not finite.
+    auto build = [&](int tile, int st) -> uint32_t {
+        unsigned char* kd = stages + st * 2 * Tl::BYTES;
         constexpr int PP = 16 / (2 * sizeof(T));  // pairs per 16-byte piece
+        const int u0 = (tile - ring_tiles) * TS;
+        uint32_t bad = 0u;
 #pragma unroll 4
         for (int j = 0; j < TS; j++) {
             const int u = u0 + j;
@@ -246,45 +259,33 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
             if (path) {
                 const float* src = rows + u * row_f;
                 const int pos = base + __popcll(path) - 1;
-                k = rope_pair(reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane], r.rope[(size_t)pos * 32 + lane]);
+                k = rope_pair(reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane],
+                              r.rope[(size_t)pos * 32 + lane]);
                 v = reinterpret_cast<const float2*>(src + (size_t)2 * H * HD)[lane];
             }
-            T kk[2] = {from_f<T>(k.x), from_f<T>(k.y)}, vv[2] = {from_f<T>(v.x), from_f<T>(v.y)};
+            const T kk[2] = {from_f<T>(k.x), from_f<T>(k.y)}, vv[2] = {from_f<T>(v.x), from_f<T>(v.y)};
             const bool odd = !isfinite(to_f(vv[0])) || !isfinite(to_f(vv[1]));
             if (__any_sync(0xffffffffu, odd)) bad |= 1u << j;
-            unsigned char* ka = kd + (j * Tl::ROW16 + ((lane / PP) ^ Tl::kswz(j))) * 16 + (lane % PP) * 2 * sizeof(T);
-            unsigned char* va =
-                kd + Tl::BYTES + (j * Tl::ROW16 + ((lane / PP) ^ Tl::vswz(j))) * 16 + (lane % PP) * 2 * sizeof(T);
-            if constexpr (F32) {
-                *reinterpret_cast<float2*>(ka) = make_float2(kk[0], kk[1]);
-                *reinterpret_cast<float2*>(va) = make_float2(vv[0], vv[1]);
-            } else {
-                reinterpret_cast<T*>(ka)[0] = kk[0], reinterpret_cast<T*>(ka)[1] = kk[1];
-                reinterpret_cast<T*>(va)[0] = vv[0], reinterpret_cast<T*>(va)[1] = vv[1];
-            }
+            T* ka = reinterpret_cast<T*>(kd + Tl::at(j, lane / PP)) + lane % PP * 2;
+            T* va = reinterpret_cast<T*>(kd + Tl::BYTES + Tl::at(j, lane / PP)) + lane % PP * 2;
+            ka[0] = kk[0], ka[1] = kk[1], va[0] = vv[0], va[1] = vv[1];
         }
         return bad;
     };
 
-    int tile = rank * WARPS + warp;
-    int seen_cur = load_seen(tile), seen_next = load_seen(tile + step);
-    uint32_t bad_cur = 0u;
-    if (tile < tiles) bad_cur = fill(tile, 0, seen_cur);
-    cp_commit();
-
     // The block's rows of q: roped, scaled (f16), split, in the order the matrix
-    // instructions take them.
+    // instructions take them.  Pair i of a fragment is row grp (i even) or grp + 8,
+    // then, 16-bit, the pair of dims 8 further on.
     {
-        constexpr int FRAGS = MT * QSTEPS * 32 / (32 * WARPS), PAIRS = F32 ? 2 : 4;
-        float2 x[FRAGS][PAIRS];
+        constexpr int FRAGS = MT * QSTEPS / WARPS, PAIRS = F32 ? 1 : 2;  // pairs of a row
+        float2 x[FRAGS][RH * PAIRS];
 #pragma unroll
         for (int f = 0; f < FRAGS; f++) {
             const int ks = (f * WARPS + warp) % QSTEPS, mt = (f * WARPS + warp) / QSTEPS;
 #pragma unroll
-            for (int i = 0; i < PAIRS; i++) {
-                // i: row grp / grp + 8, then (16-bit) the pair 8 dims on
-                const int row = mt * 16 + grp + (i & 1) * 8, t = t0 + row;
-                const int d = F32 ? (ks >> 1) * 16 + quad * 4 + (ks & 1) * 2 : ks * 16 + quad * 2 + (i >> 1) * 8;
+            for (int i = 0; i < RH * PAIRS; i++) {
+                const int row = mt * 16 + grp + (i % RH) * 8, t = t0 + row;
+                const int d = F32 ? (ks >> 1) * 16 + quad * 4 + (ks & 1) * 2 : ks * 16 + quad * 2 + (i / RH) * 8;
                 const unsigned long long path = t < nodes ? sh.path[t] : 0ull;
                 x[f][i] = make_float2(0.f, 0.f);
                 if (path) {
@@ -292,20 +293,20 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
                     x[f][i] = rope_pair(*reinterpret_cast<const float2*>(rows + t * row_f + d),
                                         r.rope[(size_t)pos * 32 + d / 2]);
                 }
-                if constexpr (std::is_same<T, __half>::value)
+                if constexpr (F16)
                     atomicMax(&sm.qmax[row], __float_as_uint(fmaxf(fabsf(x[f][i].x), fabsf(x[f][i].y))));
             }
         }
-        if constexpr (std::is_same<T, __half>::value) __syncthreads();
+        if constexpr (F16) __syncthreads();
         // f16: the row's largest |q| goes to [2^13, 2^14)
         auto up = [&](int row) {
             const int e = (int)((sm.qmax[row] >> 23) & 255u) - 127;
             return e == 128 ? 0 : min(13 - e, 100);
         };
         auto pow2 = [](int e) { return __int_as_float((e + 127) << 23); };  // e in [-114, 114]
-        if (tid < ROWS) {
+        if (tid < NODES) {
             float c = SCALE * LOG2E;
-            if constexpr (std::is_same<T, __half>::value) c *= pow2(-up(tid));
+            if constexpr (F16) c *= pow2(-up(tid));
             sm.scale[tid] = c;
         }
 #pragma unroll
@@ -313,34 +314,41 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
             const int ks = (f * WARPS + warp) % QSTEPS, mt = (f * WARPS + warp) / QSTEPS;
             if constexpr (F32) {
                 uint4 hi, lo;  // rows (grp, grp + 8) x (even, odd dim)
-                tf32_parts(x[f][0].x, hi.x, lo.x), tf32_parts(x[f][1].x, hi.y, lo.y);
-                tf32_parts(x[f][0].y, hi.z, lo.z), tf32_parts(x[f][1].y, hi.w, lo.w);
+                tf32_parts(x[f][0].x, hi.x, lo.x), tf32_parts(x[f][0].y, hi.z, lo.z);
+                if constexpr (PACK) {
+                    hi.y = lo.x, hi.w = lo.z;
+                } else {
+                    tf32_parts(x[f][1].x, hi.y, lo.y), tf32_parts(x[f][1].y, hi.w, lo.w);
+                    sm.q[Sm::QSETS - 1][mt][ks][lane] = lo;
+                }
                 sm.q[0][mt][ks][lane] = hi;
-                sm.q[1][mt][ks][lane] = lo;
             } else {
-                uint32_t p[4][NP];
+                uint32_t p[RH * 2][NP + 1];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < RH * 2; i++) {
                     float2 v = x[f][i];
-                    if constexpr (std::is_same<T, __half>::value) {
-                        const float e = pow2(up(mt * 16 + grp + (i & 1) * 8));
+                    if constexpr (F16) {
+                        const float e = pow2(up(mt * 16 + grp + (i % RH) * 8));
                         v.x *= e, v.y *= e;
                     }
+                    p[i][NP] = 0u;
                     pair_parts<T>(v.x, v.y, p[i]);
                 }
 #pragma unroll
-                for (int k = 0; k < NP; k++) sm.q[k][mt][ks][lane] = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
+                for (int k = 0; k < Sm::QSETS; k++)
+                    sm.q[k][mt][ks][lane] = PACK ? make_uint4(p[0][2 * k], p[0][2 * k + 1], p[1][2 * k], p[1][2 * k + 1])
+                                                 : make_uint4(p[0][k], p[1 % (RH * 2)][k], p[2 % (RH * 2)][k], p[3 % (RH * 2)][k]);
             }
         }
     }
     __syncthreads();
 
-    float m[MT][2], l[MT][2], o[MT][8][4], sc[MT][2];
-    int depth[MT][2];
+    float m[MT][RH], l[MT][RH], sc[MT][RH], o[MT][8][2 * RH];
+    int depth[MT][RH];
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < RH; e++) {
             const int row = mt * 16 + grp + 8 * e, t = t0 + row;
             m[mt][e] = -INFINITY, l[mt][e] = 0.f, sc[mt][e] = sm.scale[row];
             depth[mt][e] = t < nodes ? __popcll(sh.path[t]) - 1 : -1;
@@ -350,20 +358,43 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[mt][i][e] = 0.f;
+            for (int e = 0; e < 2 * RH; e++) o[mt][i][e] = 0.f;
+    uint32_t bad_cur = 0u, bad_next = 0u;
+    if (tile >= ring_tiles && tile < tiles) bad_cur = build(tile, 0);
+    if (tile + step >= ring_tiles && tile + step < tiles) bad_next = build(tile + step, 1);
+    __syncwarp();
 
+    uint32_t phase = 0u;  // parity of the next copy into a stage, a bit each
     for (int st = 0; tile < tiles; tile += step, st ^= 1) {
-        // the next tile's copies, then this one's arrival
-        uint32_t bad_next = 0u;
-        if (tile + step < tiles) bad_next = fill(tile + step, st ^ 1, seen_next);
-        cp_commit();
-        const int seen_after = load_seen(tile + 2 * step);
-        cp_wait<1>();
-        __syncwarp();
-        const unsigned char* kd = stages + st * 2 * Tl::BYTES;
+        unsigned char* kd = stages + st * 2 * Tl::BYTES;
         const uint32_t ks = smem_u32(kd), vs = ks + Tl::BYTES;
+        const bool in_ring = tile < ring_tiles;
+        int seen = -1;  // this lane's slot is seen by nodes of depth <= seen
+        bool landed = true;
+        if (in_ring) {
+            uint64_t* bar = r.wait_probe ? reinterpret_cast<uint64_t*>(&sm.never) : &full[st];
+            landed = __all_sync(0xffffffffu, mbar_wait(bar, r.wait_probe ? 0u : (phase >> st) & 1u, r.wait_limit));
+            if (!landed) {  // the tile counts as empty, and its copies land before the stage is used again
+                if (lane == 0) atomicOr(r.err, DERR_TIMEOUT);
+                mbar_wait(&full[st], (phase >> st) & 1u, WAIT_LIMIT);
+            }
+            phase ^= 1u << st;
+            if (sp_cur >= 0 && sp_cur < base && landed) seen = C - 1 - (base - sp_cur);
+            const uint32_t live = __ballot_sync(0xffffffffu, seen >= 0);
+            if (live != ~0u) {  // slots that no node sees take part with weight zero: their V must be finite
+#pragma unroll
+                for (int i = 0; i < Tl::BYTES / 512; i++) {
+                    const int e = i * 32 + lane, j = e / (HD * (int)sizeof(T) / 16);
+                    if (!((live >> j) & 1u))
+                        *reinterpret_cast<uint4*>(kd + Tl::BYTES + Tl::at(j, e % (HD * (int)sizeof(T) / 16))) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_async_smem();  // before a copy may write the stage again
+                __syncwarp();
+            }
+        }
 
-        // scores
+        // scores, columns of a lane: 16-bit slots 8 i + 2 quad, + 1; fp32 slots 8 i + quad, + 4
         float x[MT][NT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
@@ -372,13 +403,29 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[mt][i][e] = 0.f;
         if constexpr (F32) {
+            // The small products in sums of their own: what the tensor cores drop when they add is then
+            // measured against those, and not once for every product against the whole score.
+            float y[MT][NT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[mt][i][e] = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {  // 16 dims: two steps of 8, dims 4 quad .. + 3 of them in this lane
+                uint4 q[2][MT][2];
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int k = 0; k < Sm::QSETS; k++) q[e][mt][k] = sm.q[k][mt][2 * j + e][lane];
 #pragma unroll
                 for (int i = 0; i < NT; i++) {
-                    const int row = i * 8 + grp;
-                    const float4 k = *reinterpret_cast<const float4*>(
-                        kd + (row * Tl::ROW16 + ((j * 4 + quad) ^ Tl::kswz(row))) * 16);
+                    // column n is slot n / 2 + 4 (n % 2): the rows of one access phase then differ in bank
+                    const int row = i * 8 + (grp >> 1) + (grp & 1) * 4;
+                    const float4 k = *reinterpret_cast<const float4*>(kd + Tl::at(row, j * 4 + quad));
                     uint32_t hi[4], lo[4];
                     tf32_parts(k.x, hi[0], lo[0]), tf32_parts(k.y, hi[1], lo[1]);
                     tf32_parts(k.z, hi[2], lo[2]), tf32_parts(k.w, hi[3], lo[3]);
@@ -386,24 +433,27 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
                     for (int e = 0; e < 2; e++)
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
-                            const uint4 qh = sm.q[0][mt][2 * j + e][lane], ql = sm.q[1][mt][2 * j + e][lane];
-                            mma<T>(x[mt][i], ql, hi[2 * e], hi[2 * e + 1]);
-                            mma<T>(x[mt][i], qh, lo[2 * e], lo[2 * e + 1]);
-                            mma<T>(x[mt][i], qh, hi[2 * e], hi[2 * e + 1]);
+                            if constexpr (!PACK) mma<T>(y[mt][i], q[e][mt][1], hi[2 * e], hi[2 * e + 1]);
+                            mma<T>(y[mt][i], q[e][mt][0], lo[2 * e], lo[2 * e + 1]);
+                            mma<T>(x[mt][i], q[e][mt][0], hi[2 * e], hi[2 * e + 1]);
                         }
                 }
             }
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[mt][i][e] += y[mt][i][e];
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++) {  // 16 dims
                 uint32_t k[NT / 2][4];     // two groups of 8 slots each: dims 0-7, 8-15 of the first, of the second
 #pragma unroll
-                for (int i = 0; i < NT / 2; i++) {
-                    const int row = i * 16 + (lane >> 4) * 8 + (lane & 7), c = j * 2 + ((lane >> 3) & 1);
-                    ldsm4(k[i], ks + (row * Tl::ROW16 + (c ^ Tl::kswz(row))) * 16);
-                }
+                for (int i = 0; i < NT / 2; i++)
+                    ldsm4(k[i], ks + Tl::at(i * 16 + (lane >> 4) * 8 + (lane & 7), j * 2 + ((lane >> 3) & 1)));
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
+                for (int p = Sm::QSETS - 1; p >= 0; p--)
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
                         const uint4 q = sm.q[p][mt][j][lane];
@@ -412,56 +462,61 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
                     }
             }
         }
+        if constexpr (PACK) {
+#pragma unroll
+            for (int i = 0; i < NT; i++) x[0][i][0] += x[0][i][2], x[0][i][1] += x[0][i][3];
+        }
 
-        // masks: a column is slot 8 i + 2 quad + (e & 1), a row grp (e < 2) or grp + 8
+        // masks
         uint32_t bad = 0u;  // rows of V that are not finite and not seen by every node
-        const bool in_ring = tile < ring_tiles;
+        constexpr int C0 = F32 ? 1 : 2, C1 = F32 ? 4 : 1;  // a lane's columns: 8 i + C0 quad, and C1 further on
         if (!in_ring) {
             const int u0 = (tile - ring_tiles) * TS;
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
+                for (int e = 0; e < RH; e++) {
                     const int t = t0 + mt * 16 + grp + 8 * e;
                     unsigned long long path = t < nodes ? sh.path[t] : 0ull;
                     // only the last `capacity` of the path, whose earlier nodes have lower indices
                     for (int over = __popcll(path) - C; over > 0; over--) path &= path - 1ull;
-                    const uint32_t see = (uint32_t)(path >> u0) >> (2 * quad);
+                    const uint32_t see = (uint32_t)(path >> u0) >> (C0 * quad);
 #pragma unroll
                     for (int i = 0; i < NT; i++) {
                         if (!((see >> (8 * i)) & 1u)) x[mt][i][2 * e] = -INFINITY;
-                        if (!((see >> (8 * i + 1)) & 1u)) x[mt][i][2 * e + 1] = -INFINITY;
+                        if (!((see >> (8 * i + C1)) & 1u)) x[mt][i][2 * e + 1] = -INFINITY;
                     }
                 }
             bad = bad_cur;
-        } else if (!__all_sync(0xffffffffu, seen_cur >= max_depth)) {
+        } else if (!__all_sync(0xffffffffu, seen >= max_depth)) {
 #pragma unroll
             for (int i = 0; i < NT; i++) {
-                const int s0 = __shfl_sync(0xffffffffu, seen_cur, 8 * i + 2 * quad);
-                const int s1 = __shfl_sync(0xffffffffu, seen_cur, 8 * i + 2 * quad + 1);
+                const int s0 = __shfl_sync(0xffffffffu, seen, 8 * i + C0 * quad);
+                const int s1 = __shfl_sync(0xffffffffu, seen, 8 * i + C0 * quad + C1);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
+                    for (int e = 0; e < RH; e++) {
                         if (depth[mt][e] > s0 || s0 < 0) x[mt][i][2 * e] = -INFINITY;
                         if (depth[mt][e] > s1 || s1 < 0) x[mt][i][2 * e + 1] = -INFINITY;
                     }
             }
-            // (dead slots hold zeros; these are the ones that only some nodes see)
-            uint32_t some = __ballot_sync(0xffffffffu, seen_cur >= 0 && seen_cur < max_depth) & (TS == 32 ? ~0u : 0xFFFFu);
+            // slots that only some nodes see
+            uint32_t some = __ballot_sync(0xffffffffu, seen >= 0 && seen < max_depth) & (TS == 32 ? ~0u : 0xFFFFu);
             for (; some; some &= some - 1u) {
                 const int j = __ffs(some) - 1;
-                const T* v = reinterpret_cast<const T*>(kd + Tl::BYTES + j * HD * sizeof(T));
-                if (__any_sync(0xffffffffu, !isfinite(to_f(v[lane])) || !isfinite(to_f(v[lane + 32])))) bad |= 1u << j;
+                const T* v = reinterpret_cast<const T*>(kd + Tl::BYTES + j * 128);  // in any order
+                const T* w = F32 ? reinterpret_cast<const T*>(kd + Tl::BYTES + Tl::HALF + j * 128) : v + 32;
+                if (__any_sync(0xffffffffu, !isfinite(to_f(v[lane])) || !isfinite(to_f(w[lane])))) bad |= 1u << j;
             }
         }
 
         // weights
-        float alpha[MT][2];
+        float alpha[MT][RH];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
+            for (int e = 0; e < RH; e++) {
                 float top = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < NT; i++) top = fmaxf(top, fmaxf(x[mt][i][2 * e], x[mt][i][2 * e + 1]));
@@ -484,43 +539,48 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
             }
         if (bad) {
             // Rows of V that are not finite reach only the nodes that see them: added one by one, then set to
-            // zero for the products below (whose weights of the other nodes are zero, and 0 * inf is not).
+            // zero for the products below (whose weights of the other nodes are zero, and 0 * inf is not).  The
+            // weights pass through the stage's K, which is no longer needed.
+            float* pw = reinterpret_cast<float*>(kd);
+            __syncwarp();
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                for (int i = 0; i < 8; i++)
+                for (int e = 0; e < RH; e++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[mt][i][e] *= alpha[mt][e >> 1];
-                alpha[mt][0] = alpha[mt][1] = 1.f;
-                for (uint32_t b = bad; b; b &= b - 1u) {
-                    const int j = __ffs(b) - 1;
-                    float p0 = 0.f, p1 = 0.f;
+                    for (int i = 0; i < NT; i++) {
+                        pw[(mt * 16 + grp + 8 * e) * TS + 8 * i + C0 * quad] = x[mt][i][2 * e];
+                        pw[(mt * 16 + grp + 8 * e) * TS + 8 * i + C0 * quad + C1] = x[mt][i][2 * e + 1];
+                    }
+            __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < NT; i++)
-                        if (i == (j >> 3)) {
-                            const float a0 = x[mt][i][0], a1 = x[mt][i][1], a2 = x[mt][i][2], a3 = x[mt][i][3];
-                            p0 = (j & 1) ? a1 : a0, p1 = (j & 1) ? a3 : a2;
-                        }
-                    p0 = __shfl_sync(0xffffffffu, p0, (lane & ~3) | ((j & 7) >> 1));
-                    p1 = __shfl_sync(0xffffffffu, p1, (lane & ~3) | ((j & 7) >> 1));
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
+                for (int e = 0; e < RH; e++) {
 #pragma unroll
-                        for (int f = 0; f < 2; f++) {
-                            const int d = F32 ? 16 * quad + 8 * f + i : 8 * i + 2 * quad + f;
-                            const int at = (j * Tl::ROW16 + ((d * (int)sizeof(T) / 16) ^ Tl::vswz(j))) * 16 +
-                                           d * (int)sizeof(T) % 16;
-                            const float v = to_f(*reinterpret_cast<const T*>(kd + Tl::BYTES + at));
-                            if (p0 != 0.f) o[mt][i][f] = fmaf(p0, v, o[mt][i][f]);
-                            if (p1 != 0.f) o[mt][i][2 + f] = fmaf(p1, v, o[mt][i][2 + f]);
-                        }
+                    for (int i = 0; i < 8; i++) o[mt][i][2 * e] *= alpha[mt][e], o[mt][i][2 * e + 1] *= alpha[mt][e];
+                    alpha[mt][e] = 1.f;
+                    for (uint32_t b = bad; b; b &= b - 1u) {
+                        const int j = __ffs(b) - 1;
+                        const float p = pw[(mt * 16 + grp + 8 * e) * TS + j];
+                        if (p != 0.f)
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+#pragma unroll
+                                for (int f = 0; f < 2; f++) {
+                                    const int d = F32 ? 32 * (i >> 2) + 16 * f + 4 * quad + (i & 3) : 8 * i + 2 * quad + f;
+                                    const T* v = reinterpret_cast<const T*>(kd + Tl::BYTES + Tl::at(j, d * (int)sizeof(T) / 16));
+                                    o[mt][i][2 * e + f] = fmaf(p, to_f(v[d % (16 / (int)sizeof(T))]), o[mt][i][2 * e + f]);
+                                }
+                    }
                 }
-            }
             __syncwarp();
             for (uint32_t b = bad; b; b &= b - 1u) {
-                unsigned char* row = stages + st * 2 * Tl::BYTES + Tl::BYTES + (__ffs(b) - 1) * HD * sizeof(T);
-                if (lane < Tl::ROW16) reinterpret_cast<uint4*>(row)[lane] = make_uint4(0u, 0u, 0u, 0u);
+                const int j = __ffs(b) - 1;
+                if (lane < HD * (int)sizeof(T) / 16)
+                    *reinterpret_cast<uint4*>(kd + Tl::BYTES + Tl::at(j, lane)) = make_uint4(0u, 0u, 0u, 0u);
             }
+            fence_async_smem();
             __syncwarp();
         }
 
@@ -535,23 +595,26 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
                 for (int e = 0; e < 4; e++) ot[i][e] = 0.f;
             if constexpr (F32) {
 #pragma unroll
-                for (int i = 0; i < NT; i++) {  // 8 slots: step depth k = quad is slot 2 quad, quad + 4 slot 2 quad + 1
+                for (int i = 0; i < NT; i++) {  // 8 slots
                     uint4 ph, pl;
-                    tf32_parts(x[mt][i][0], ph.x, pl.x), tf32_parts(x[mt][i][2], ph.y, pl.y);
-                    tf32_parts(x[mt][i][1], ph.z, pl.z), tf32_parts(x[mt][i][3], ph.w, pl.w);
+                    tf32_parts(x[mt][i][0], ph.x, pl.x), tf32_parts(x[mt][i][1], ph.z, pl.z);
+                    if constexpr (PACK)
+                        ph.y = pl.x, ph.w = pl.z;
+                    else
+                        tf32_parts(x[mt][i][2], ph.y, pl.y), tf32_parts(x[mt][i][3], ph.w, pl.w);
+                    // column n of group 4 c + f is dim 32 c + 4 (n / 2 + 4 (n % 2)) + f
+                    const int pn = (grp >> 1) + (grp & 1) * 4;
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {  // dims 8 grp + 4 c .. + 3: one for each of four column groups
-                        const int j0 = i * 8 + 2 * quad, j1 = j0 + 1;
-                        const float4 a = *reinterpret_cast<const float4*>(
-                            kd + Tl::BYTES + (j0 * Tl::ROW16 + ((2 * grp + c) ^ Tl::vswz(j0))) * 16);
-                        const float4 b = *reinterpret_cast<const float4*>(
-                            kd + Tl::BYTES + (j1 * Tl::ROW16 + ((2 * grp + c) ^ Tl::vswz(j1))) * 16);
+                    for (int c = 0; c < 2; c++) {
+                        const float4 a = *reinterpret_cast<const float4*>(kd + Tl::BYTES + Tl::at(i * 8 + quad, 8 * c + pn));
+                        const float4 b =
+                            *reinterpret_cast<const float4*>(kd + Tl::BYTES + Tl::at(i * 8 + quad + 4, 8 * c + pn));
                         const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
                         for (int f = 0; f < 4; f++) {
                             uint32_t h0, l0, h1, l1;
                             tf32_parts(av[f], h0, l0), tf32_parts(bv[f], h1, l1);
-                            mma<T>(ot[4 * c + f], pl, h0, h1);
+                            if constexpr (!PACK) mma<T>(ot[4 * c + f], pl, h0, h1);
                             mma<T>(ot[4 * c + f], ph, l0, l1);
                             mma<T>(ot[4 * c + f], ph, h0, h1);
                         }
@@ -560,20 +623,24 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
             } else {
 #pragma unroll
                 for (int i = 0; i < NT / 2; i++) {  // 16 slots
-                    uint32_t pp[4][NP];
+                    uint32_t pp[RH * 2][NP + 1];
 #pragma unroll
                     for (int f = 0; f < 2; f++) {
-                        pair_parts<T>(x[mt][2 * i + f][0], x[mt][2 * i + f][1], pp[2 * f]);
-                        pair_parts<T>(x[mt][2 * i + f][2], x[mt][2 * i + f][3], pp[2 * f + 1]);
+#pragma unroll
+                        for (int e = 0; e < RH; e++) {
+                            pp[RH * f + e][NP] = 0u;
+                            pair_parts<T>(x[mt][2 * i + f][2 * e], x[mt][2 * i + f][2 * e + 1], pp[RH * f + e]);
+                        }
                     }
 #pragma unroll
                     for (int c = 0; c < 4; c++) {  // 16 dims
                         uint32_t v[4];
-                        const int row = i * 16 + (lane & 15);
-                        ldsm4t(v, vs + (row * Tl::ROW16 + ((2 * c + (lane >> 4)) ^ Tl::vswz(row))) * 16);
+                        ldsm4t(v, vs + Tl::at(i * 16 + (lane & 15), 2 * c + (lane >> 4)));
 #pragma unroll
-                        for (int p = NP - 1; p >= 0; p--) {
-                            const uint4 a = make_uint4(pp[0][p], pp[1][p], pp[2][p], pp[3][p]);
+                        for (int p = Sm::QSETS - 1; p >= 0; p--) {
+                            const uint4 a =
+                                PACK ? make_uint4(pp[0][2 * p], pp[0][2 * p + 1], pp[1][2 * p], pp[1][2 * p + 1])
+                                     : make_uint4(pp[0][p], pp[1 % (RH * 2)][p], pp[2 % (RH * 2)][p], pp[3 % (RH * 2)][p]);
                             mma<T>(ot[2 * c], a, v[0], v[1]);
                             mma<T>(ot[2 * c + 1], a, v[2], v[3]);
                         }
@@ -583,40 +650,51 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
 #pragma unroll
             for (int i = 0; i < 8; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[mt][i][e] = fmaf(o[mt][i][e], alpha[mt][e >> 1], ot[i][e]);
+                for (int e = 0; e < 2 * RH; e++)
+                    o[mt][i][e] = fmaf(o[mt][i][e], alpha[mt][e >> 1], PACK ? ot[i][e] + ot[i][e + 2 * (PACK ? 1 : 0)] : ot[i][e]);
         }
-        __syncwarp();  // before the stage is filled again
-        seen_cur = seen_next, seen_next = seen_after, bad_cur = bad_next;
+        __syncwarp();  // every lane is done with the stage
+        sp_cur = sp_next, bad_cur = bad_next, bad_next = 0u;
+        const int ahead = tile + 2 * step;
+        sp_next = slot_position(ahead);
+        if (ahead < ring_tiles)
+            fetch(ahead, st);
+        else if (ahead < tiles) {
+            bad_next = build(ahead, st);
+            __syncwarp();
+        }
     }
-    cp_wait<0>();
-    __syncwarp();
 
     // Join: each warp's rows to its own stages, then the warps' into the first.
-    float* mine = reinterpret_cast<float*>(sm.stage[warp][0]);
+    float* mine = reinterpret_cast<float*>(stages);
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < RH; e++) {
             const int row = mt * 16 + grp + 8 * e;
             float sum = l[mt][e];
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             if (quad == 0) sm.m[warp][row] = m[mt][e], sm.l[warp][row] = sum;
+            if constexpr (F32) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if constexpr (F32) {
-                    mine[row * HD + 16 * quad + i] = o[mt][i][2 * e];
-                    mine[row * HD + 16 * quad + 8 + i] = o[mt][i][2 * e + 1];
-                } else {
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int f = 0; f < 2; f++)
+                        *reinterpret_cast<float4*>(mine + row * HD + 32 * c + 16 * f + 4 * quad) =
+                            make_float4(o[mt][4 * c][2 * e + f], o[mt][4 * c + 1][2 * e + f],
+                                        o[mt][4 * c + 2][2 * e + f], o[mt][4 * c + 3][2 * e + f]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
                     *reinterpret_cast<float2*>(mine + row * HD + 8 * i + 2 * quad) =
                         make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
-                }
             }
         }
     __syncthreads();
     const size_t out_row = (size_t)H * HD;
     float* dst = out + ((size_t)item * nodes + t0) * out_row + h * HD;
-    for (int i = tid; i < ROWS * 16; i += 32 * WARPS) {
+    for (int i = tid; i < NODES * 16; i += 32 * WARPS) {
         const int row = i >> 4, d = (i & 15) * 4;
         float top = sm.m[0][row];
 #pragma unroll
@@ -649,7 +727,7 @@ __global__ void __launch_bounds__(32 * WARPS) tree_attend_kernel(RingView r, int
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     // rows rank, rank + splits, .. from every block of the cluster
-    for (int i = tid; i < ROWS / splits * 16; i += 32 * WARPS) {
+    for (int i = tid; i < NODES / splits * 16; i += 32 * WARPS) {
         const int row = (i >> 4) * splits + rank, d = (i & 15) * 4;
         float top = -INFINITY;
         for (int b = 0; b < splits; b++) top = fmaxf(top, *cluster.map_shared_rank(&sm.m[0][row], b));
@@ -731,10 +809,35 @@ __global__ void __launch_bounds__(1024) tree_commit_kernel(RingView r, int n, in
     }
 }
 
-template <typename T, int MT>
+// The rings of one layer as rows of 64 elements, for boxes of one tile's slots: 128
+// bytes of each, at x = 0 (or 32 floats), so the 16-byte rule on x holds.
+template <typename T>
+bool make_ring_map(CUtensorMap* m, const RingView& r) {
+    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    const cuuint64_t dims[2] = {HD, (cuuint64_t)r.streams * 2 * r.heads * r.capacity};
+    if (!fn || dims[1] > 0x7fffffffull) return false;
+    const cuuint64_t strides[1] = {HD * sizeof(T)};
+    const cuuint32_t box[2] = {128 / sizeof(T), (cuuint32_t)Tile<T>::SLOTS}, estr[2] = {1, 1};
+    const CUtensorMapDataType type = sizeof(T) == 4                    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return fn(m, type, 2, r.kv, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int MT, bool PACK>
 cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* streams, const int32_t* positions,
                       const int32_t* parents, const float* qkv, float* out, cudaStream_t st) {
-    constexpr int smem = sizeof(TreeSmem<T, MT>);
+    using Sm = TreeSmem<T, MT, PACK>;
+    constexpr int smem = sizeof(Sm);
+    const auto kernel = tree_attend_kernel<T, MT, PACK>;
     // the opt-in to more than 48 KB of shared memory, once per device
     static std::atomic<uint64_t> opted{0};
     int dev = 0;
@@ -742,15 +845,17 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
     if (e != cudaSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
     if (dev > 63 || !(opted.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(tree_attend_kernel<T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
         opted.fetch_or(bit, std::memory_order_release);
     }
-    const int qtiles = (nodes + 16 * MT - 1) / (16 * MT);
+    CUtensorMap map;
+    if (!make_ring_map<T>(&map, r)) return cudaErrorInvalidValue;
+    const int qtiles = (nodes + Sm::NODES - 1) / Sm::NODES;
     const int tiles = (r.capacity + Tile<T>::SLOTS - 1) / Tile<T>::SLOTS + (nodes + Tile<T>::SLOTS - 1) / Tile<T>::SLOTS;
     const int blocks = n * r.heads * qtiles;
     int splits = 1;
-    while (splits < 8 && blocks * splits < 2 * 148 && splits * WARPS < tiles) splits *= 2;
+    while (splits < 8 && blocks * splits < SPLIT_BELOW && splits * WARPS < tiles) splits *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(blocks * splits);
     cfg.blockDim = dim3(32 * WARPS);
@@ -761,15 +866,15 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
     attr.val.clusterDim = {(unsigned)splits, 1, 1};
     cfg.attrs = &attr;
     cfg.numAttrs = splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, tree_attend_kernel<T, MT>, r, nodes, qtiles, splits, streams, positions, parents,
-                              qkv, out);
+    return cudaLaunchKernelEx(&cfg, kernel, map, r, nodes, qtiles, splits, streams, positions, parents, qkv, out);
 }
 
 template <typename T>
 cudaError_t attend_t(const RingView& r, int n, int nodes, const int32_t* streams, const int32_t* positions,
                      const int32_t* parents, const float* qkv, float* out, cudaStream_t st) {
-    return nodes <= 16 ? attend_mt<T, 1>(r, n, nodes, streams, positions, parents, qkv, out, st)
-                       : attend_mt<T, 2>(r, n, nodes, streams, positions, parents, qkv, out, st);
+    if (nodes <= 8) return attend_mt<T, 1, true>(r, n, nodes, streams, positions, parents, qkv, out, st);
+    if (nodes <= 16) return attend_mt<T, 1, false>(r, n, nodes, streams, positions, parents, qkv, out, st);
+    return attend_mt<T, 2, false>(r, n, nodes, streams, positions, parents, qkv, out, st);
 }
 
 template <typename T>
