@@ -16,6 +16,9 @@
 #include <cudaTypedefs.h>
 
 #include <atomic>
+#ifdef TUNE
+#include <stdlib.h>
+#endif
 #include <type_traits>
 
 #include "mb_ptx.cuh"
@@ -143,7 +146,10 @@ __device__ __forceinline__ void pair_parts(float x, float y, uint32_t* p) {
 // The rows of a matrix tile are 16 nodes, or (PACK, at most 8 nodes) two parts of
 // the same 8 nodes, whose products the lane that holds both adds up.
 constexpr int WARPS = 4, STAGES = 2;
-#ifndef SPLIT_BELOW
+#ifdef TUNE
+static int tune(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
+#define SPLIT_BELOW tune("SPLIT_BELOW", 296)
+#else
 #define SPLIT_BELOW 296
 #endif
 
@@ -194,8 +200,12 @@ __global__ void __launch_bounds__(32 * WARPS)
     const int s = streams[item], base = positions[item];
     const bool in_range = s >= 0 && s < r.streams && base >= 0;
     const int window = in_range ? min(base, C) : 0;
-    const int ring_tiles = (window + TS - 1) / TS, tiles = ring_tiles + (nodes + TS - 1) / TS;
+    const int ring_tiles = (window + TS - 1) / TS, tree_tiles = (nodes + TS - 1) / TS;
     const int step = splits * WARPS;
+    // Warp w of the cluster takes tiles w, w + step, .. of: one ring tile for each warp, the tree's tiles (at most
+    // WARPS, so no warp builds one later than as its second), the ring's other tiles.
+    const int first = min(step, ring_tiles), tiles = ring_tiles + tree_tiles;
+    auto ring_tile = [&](int tile) { return tile < first ? tile : tile >= first + tree_tiles && tile < tiles ? tile - tree_tiles : -1; };
     const size_t plane = in_range ? ((size_t)s * 2 * H + h) * C : 0;  // K's rows in the map; V's lie H * C on
     const int32_t* sp = r.slot_pos + (in_range ? (size_t)s * C : 0);
     uint64_t* const full = reinterpret_cast<uint64_t*>(sm.full[warp]);
@@ -203,7 +213,7 @@ __global__ void __launch_bounds__(32 * WARPS)
     auto fetch = [&](int tile, int st) {
         if (lane == 0) {
             unsigned char* kd = stages + st * 2 * Tl::BYTES;
-            const int row = (int)plane + tile * TS;
+            const int row = (int)plane + ring_tile(tile) * TS;
             mbar_expect_tx(&full[st], 2 * Tl::BYTES);
 #pragma unroll
             for (int c = 0; c < Tl::BYTES / Tl::HALF; c++) {
@@ -213,8 +223,8 @@ __global__ void __launch_bounds__(32 * WARPS)
         }
     };
     auto slot_position = [&](int tile) {
-        const int j = tile * TS + (lane & (TS - 1));
-        return j < window ? sp[j] : -1;
+        const int j = ring_tile(tile) * TS + (lane & (TS - 1));
+        return j >= 0 && j < window ? sp[j] : -1;
     };
     int tile = rank * WARPS + warp;
     int sp_cur = slot_position(tile), sp_next = slot_position(tile + step);
@@ -224,8 +234,8 @@ __global__ void __launch_bounds__(32 * WARPS)
         fence_mbar_init();
     }
     __syncwarp();
-    if (tile < ring_tiles) fetch(tile, 0);
-    if (tile + step < ring_tiles) fetch(tile + step, 1);
+    if (ring_tile(tile) >= 0) fetch(tile, 0);
+    if (ring_tile(tile + step) >= 0) fetch(tile + step, 1);
     if (warp == 0) tree_shape(sm.shape, parents + (size_t)item * nodes, nodes, lane);
     if (tid < NODES) sm.qmax[tid] = 0u;
     __syncthreads();
@@ -237,39 +247,59 @@ __global__ void __launch_bounds__(32 * WARPS)
     if (absent || why) {
         if (why && blockIdx.x % (splits * qtiles * H) == 0 && tid == 0) atomicOr(r.err, why);
         // no block leaves its shared memory while copies into it are under way
-        if (tile < ring_tiles) mbar_wait(&full[0], 0, WAIT_LIMIT);
-        if (tile + step < ring_tiles) mbar_wait(&full[1], 0, WAIT_LIMIT);
+        if (ring_tile(tile) >= 0) mbar_wait(&full[0], 0, WAIT_LIMIT);
+        if (ring_tile(tile + step) >= 0) mbar_wait(&full[1], 0, WAIT_LIMIT);
         return;
     }
     const size_t row_f = (size_t)3 * H * HD;
     const float* rows = qkv + (size_t)item * nodes * row_f + h * HD;
 
-    // Builds a tile of the tree's own K and V, one row at a time: lane i ropes dims
-    // (2 i, 2 i + 1).  Returns the nodes whose V is not finite.
+    // Builds a tile of the tree's own K and V, eight rows' loads at a time: lane i
+    // ropes dims (2 i, 2 i + 1).  Returns the nodes whose V is not finite.  (Absent
+    // nodes read row 0 and store zeros.)
     auto build = [&](int tile, int st) -> uint32_t {
         unsigned char* kd = stages + st * 2 * Tl::BYTES;
-        constexpr int PP = 16 / (2 * sizeof(T));  // pairs per 16-byte piece
-        const int u0 = (tile - ring_tiles) * TS;
+        constexpr int PP = 16 / (2 * sizeof(T)), RB = 8;  // pairs per 16-byte piece, rows per batch
+        const int u0 = (tile - first) * TS;
         uint32_t bad = 0u;
-#pragma unroll 4
-        for (int j = 0; j < TS; j++) {
-            const int u = u0 + j;
-            float2 k = make_float2(0.f, 0.f), v = k;
-            const unsigned long long path = u < nodes ? sh.path[u] : 0ull;
-            if (path) {
-                const float* src = rows + u * row_f;
-                const int pos = base + __popcll(path) - 1;
-                k = rope_pair(reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane],
-                              r.rope[(size_t)pos * 32 + lane]);
-                v = reinterpret_cast<const float2*>(src + (size_t)2 * H * HD)[lane];
+#pragma unroll 1
+        for (int j0 = 0; j0 < TS && u0 + j0 < nodes; j0 += RB) {
+            float2 k[RB], v[RB], cs[RB];
+            uint32_t on = 0u;
+#pragma unroll
+            for (int j = 0; j < RB; j++) {
+                const int u = u0 + j0 + j;
+                const unsigned long long path = u < nodes ? sh.path[u] : 0ull;
+                const float* src = rows + (path ? u : 0) * row_f;
+                const int pos = base + (path ? __popcll(path) - 1 : 0);
+                on |= path ? 1u << j : 0u;
+                k[j] = reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane];
+                v[j] = reinterpret_cast<const float2*>(src + (size_t)2 * H * HD)[lane];
+                cs[j] = r.rope[(size_t)pos * 32 + lane];
             }
-            const T kk[2] = {from_f<T>(k.x), from_f<T>(k.y)}, vv[2] = {from_f<T>(v.x), from_f<T>(v.y)};
-            const bool odd = !isfinite(to_f(vv[0])) || !isfinite(to_f(vv[1]));
-            if (__any_sync(0xffffffffu, odd)) bad |= 1u << j;
-            T* ka = reinterpret_cast<T*>(kd + Tl::at(j, lane / PP)) + lane % PP * 2;
-            T* va = reinterpret_cast<T*>(kd + Tl::BYTES + Tl::at(j, lane / PP)) + lane % PP * 2;
-            ka[0] = kk[0], ka[1] = kk[1], va[0] = vv[0], va[1] = vv[1];
+#pragma unroll
+            for (int j = 0; j < RB; j++) {
+                const float2 kr = (on >> j) & 1u ? rope_pair(k[j], cs[j]) : make_float2(0.f, 0.f);
+                const float2 vr = (on >> j) & 1u ? v[j] : make_float2(0.f, 0.f);
+                alignas(8) const T kk[2] = {from_f<T>(kr.x), from_f<T>(kr.y)}, vv[2] = {from_f<T>(vr.x), from_f<T>(vr.y)};
+                const bool odd = !isfinite(to_f(vv[0])) || !isfinite(to_f(vv[1]));
+                if (__any_sync(0xffffffffu, odd)) bad |= 1u << (j0 + j);
+                T* ka = reinterpret_cast<T*>(kd + Tl::at(j0 + j, lane / PP)) + lane % PP * 2;
+                T* va = reinterpret_cast<T*>(kd + Tl::BYTES + Tl::at(j0 + j, lane / PP)) + lane % PP * 2;
+                if constexpr (F32) {
+                    *reinterpret_cast<float2*>(ka) = make_float2(kk[0], kk[1]);
+                    *reinterpret_cast<float2*>(va) = make_float2(vv[0], vv[1]);
+                } else {
+                    *reinterpret_cast<uint32_t*>(ka) = *reinterpret_cast<const uint32_t*>(kk);
+                    *reinterpret_cast<uint32_t*>(va) = *reinterpret_cast<const uint32_t*>(vv);
+                }
+            }
         }
+        // the rest of the tile: weight zero, so V has to be finite there
+        for (int j = max(0, (nodes - u0 + RB - 1) / RB * RB); j < TS; j++)
+            if (lane < HD * (int)sizeof(T) / 16)
+                *reinterpret_cast<uint4*>(kd + Tl::BYTES + Tl::at(j, lane)) = make_uint4(0u, 0u, 0u, 0u);
+        fence_async_smem();  // before a copy may write the stage
         return bad;
     };
 
@@ -278,25 +308,30 @@ __global__ void __launch_bounds__(32 * WARPS)
     // then, 16-bit, the pair of dims 8 further on.
     {
         constexpr int FRAGS = MT * QSTEPS / WARPS, PAIRS = F32 ? 1 : 2;  // pairs of a row
-        float2 x[FRAGS][RH * PAIRS];
+        float2 x[FRAGS][RH * PAIRS], cs[FRAGS][RH * PAIRS];
+        bool on[FRAGS][RH * PAIRS];
 #pragma unroll
-        for (int f = 0; f < FRAGS; f++) {
+        for (int f = 0; f < FRAGS; f++) {  // (every load before the first use; absent nodes read row 0)
             const int ks = (f * WARPS + warp) % QSTEPS, mt = (f * WARPS + warp) / QSTEPS;
 #pragma unroll
             for (int i = 0; i < RH * PAIRS; i++) {
-                const int row = mt * 16 + grp + (i % RH) * 8, t = t0 + row;
+                const int t = t0 + mt * 16 + grp + (i % RH) * 8;
                 const int d = F32 ? (ks >> 1) * 16 + quad * 4 + (ks & 1) * 2 : ks * 16 + quad * 2 + (i / RH) * 8;
                 const unsigned long long path = t < nodes ? sh.path[t] : 0ull;
-                x[f][i] = make_float2(0.f, 0.f);
-                if (path) {
-                    const int pos = base + __popcll(path) - 1;
-                    x[f][i] = rope_pair(*reinterpret_cast<const float2*>(rows + t * row_f + d),
-                                        r.rope[(size_t)pos * 32 + d / 2]);
-                }
-                if constexpr (F16)
-                    atomicMax(&sm.qmax[row], __float_as_uint(fmaxf(fabsf(x[f][i].x), fabsf(x[f][i].y))));
+                on[f][i] = path != 0ull;
+                x[f][i] = *reinterpret_cast<const float2*>(rows + (path ? t : 0) * row_f + d);
+                cs[f][i] = r.rope[(size_t)(base + (path ? __popcll(path) - 1 : 0)) * 32 + d / 2];
             }
         }
+#pragma unroll
+        for (int f = 0; f < FRAGS; f++)
+#pragma unroll
+            for (int i = 0; i < RH * PAIRS; i++) {
+                x[f][i] = on[f][i] ? rope_pair(x[f][i], cs[f][i]) : make_float2(0.f, 0.f);
+                if constexpr (F16)
+                    atomicMax(&sm.qmax[(f * WARPS + warp) / QSTEPS * 16 + grp + (i % RH) * 8],
+                              __float_as_uint(fmaxf(fabsf(x[f][i].x), fabsf(x[f][i].y))));
+            }
         if constexpr (F16) __syncthreads();
         // f16: the row's largest |q| goes to [2^13, 2^14)
         auto up = [&](int row) {
@@ -360,15 +395,15 @@ __global__ void __launch_bounds__(32 * WARPS)
 #pragma unroll
             for (int e = 0; e < 2 * RH; e++) o[mt][i][e] = 0.f;
     uint32_t bad_cur = 0u, bad_next = 0u;
-    if (tile >= ring_tiles && tile < tiles) bad_cur = build(tile, 0);
-    if (tile + step >= ring_tiles && tile + step < tiles) bad_next = build(tile + step, 1);
+    if (tile < tiles && ring_tile(tile) < 0) bad_cur = build(tile, 0);
+    if (tile + step < tiles && ring_tile(tile + step) < 0) bad_next = build(tile + step, 1);
     __syncwarp();
 
     uint32_t phase = 0u;  // parity of the next copy into a stage, a bit each
     for (int st = 0; tile < tiles; tile += step, st ^= 1) {
         unsigned char* kd = stages + st * 2 * Tl::BYTES;
         const uint32_t ks = smem_u32(kd), vs = ks + Tl::BYTES;
-        const bool in_ring = tile < ring_tiles;
+        const bool in_ring = ring_tile(tile) >= 0;
         int seen = -1;  // this lane's slot is seen by nodes of depth <= seen
         bool landed = true;
         if (in_ring) {
@@ -471,7 +506,7 @@ __global__ void __launch_bounds__(32 * WARPS)
         uint32_t bad = 0u;  // rows of V that are not finite and not seen by every node
         constexpr int C0 = F32 ? 1 : 2, C1 = F32 ? 4 : 1;  // a lane's columns: 8 i + C0 quad, and C1 further on
         if (!in_ring) {
-            const int u0 = (tile - ring_tiles) * TS;
+            const int u0 = (tile - first) * TS;
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -657,12 +692,7 @@ __global__ void __launch_bounds__(32 * WARPS)
         sp_cur = sp_next, bad_cur = bad_next, bad_next = 0u;
         const int ahead = tile + 2 * step;
         sp_next = slot_position(ahead);
-        if (ahead < ring_tiles)
-            fetch(ahead, st);
-        else if (ahead < tiles) {
-            bad_next = build(ahead, st);
-            __syncwarp();
-        }
+        if (ring_tile(ahead) >= 0) fetch(ahead, st);
     }
 
     // Join: each warp's rows to its own stages, then the warps' into the first.
