@@ -57,6 +57,8 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
                  : "memory");
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // d[16 x 8] += a b with fp32 accumulation: bf16 or f16 operands 16 deep, tf32 operands 8 deep
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -111,6 +113,14 @@ __device__ __forceinline__ void tf32_parts(float x, uint32_t& hi, uint32_t& lo) 
     lo = to_tf32(x - __uint_as_float(hi));
 }
 
+// The same for K and V, of which there are many: by truncation, three full-rate operations.  (What the second part
+// leaves is below 2^-21 of x; and with the other operand's parts rounded to nearest, the product lo lo that is
+// left out has no sign of its own.)
+__device__ __forceinline__ void tf32_cut(float x, uint32_t& hi, uint32_t& lo) {
+    hi = __float_as_uint(x) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xFFFFE000u;
+}
+
 // p[i]: the packed 16-bit parts of (x, y), largest first
 template <typename T>
 __device__ __forceinline__ void pair_parts(float x, float y, uint32_t* p) {
@@ -145,11 +155,17 @@ __device__ __forceinline__ void pair_parts(float x, float y, uint32_t* p) {
 //
 // The rows of a matrix tile are 16 nodes, or (PACK, at most 8 nodes) two parts of
 // the same 8 nodes, whose products the lane that holds both adds up.
-constexpr int WARPS = 4, STAGES = 2;
+constexpr int WARPS = 4, STAGES = 2, SORT_MAX = 256;
 #ifdef TUNE
 static int tune(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
 #define SPLIT_BELOW tune("SPLIT_BELOW", 296)
+#define PFD tune("PFD", 0)
+#define SORT (tune("SORT", 1) && n > 1 && n <= SORT_MAX)
+#define PREFETCH prefetch_dist
 #else
+#define PREFETCH 0
+#define PFD 0
+#define SORT (n > 1 && n <= SORT_MAX)
 #define SPLIT_BELOW 296
 #endif
 
@@ -176,12 +192,14 @@ struct alignas(1024) TreeSmem {
     float m[WARPS][NODES], l[WARPS][NODES];                  // [0]: the block's after the join
     float scale[NODES];                                      // of a score in units of log2
     unsigned int qmax[NODES];
+    unsigned int bad[WARPS];                                 // nodes of the warp's tree tile whose V is not finite
     TreeShape shape;
+    int window[SORT_MAX], item;                              // of every item; the block's
 };
 
 template <typename T, int MT, bool PACK>
 __global__ void __launch_bounds__(32 * WARPS)
-    tree_attend_kernel(const __grid_constant__ CUtensorMap map, RingView r, int nodes, int qtiles, int splits,
+    tree_attend_kernel(const __grid_constant__ CUtensorMap map, RingView r, int n, int nodes, int qtiles, int splits, bool sort, int prefetch_dist,
                        const int32_t* __restrict__ streams, const int32_t* __restrict__ positions,
                        const int32_t* __restrict__ parents, const float* __restrict__ qkv, float* __restrict__ out) {
     using Tl = Tile<T>;
@@ -194,10 +212,44 @@ __global__ void __launch_bounds__(32 * WARPS)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, quad = lane & 3;
     const int H = r.heads, C = r.capacity;
     const int rank = blockIdx.x % splits, qt = (blockIdx.x / splits) % qtiles;
-    const int h = (blockIdx.x / splits / qtiles) % H, item = blockIdx.x / splits / qtiles / H;
+    const int h = (blockIdx.x / splits / qtiles) % H;
+    int item = blockIdx.x / splits / qtiles / H;
+    if (sort) {
+        // Blocks start in the order of their numbers, so the longest windows come first and the short ones fill
+        // the gaps at the end: this block takes the item that `item` others come before.
+        const int place = item;
+        for (int i = tid; i < n; i += 32 * WARPS) sm.window[i] = min(max(positions[i], 0), C);
+        __syncthreads();
+        for (int i = tid; i < n; i += 32 * WARPS) {
+            const int w = sm.window[i];
+            int ahead = 0;
+            for (int j = 0; j < n; j++) ahead += sm.window[j] > w || (sm.window[j] == w && j < i);
+            if (ahead == place) sm.item = i;
+        }
+        __syncthreads();
+        item = sm.item;
+    }
 
-    // The ring's first tiles are on their way before the tree is looked at.
+    // Everything that does not wait for the tree is on its way before the tree is looked at: the block's rows of q
+    // (in the order the matrix instructions take them: pair i of a fragment is row grp (i even) or grp + 8, then,
+    // 16-bit, the pair of dims 8 further on), the tree's own K and V into L2, the ring's first tiles.
+    constexpr int FRAGS = MT * QSTEPS / WARPS, PAIRS = F32 ? 1 : 2;  // pairs of a row
+    const int t0 = qt * NODES;
+    const size_t row_f = (size_t)3 * H * HD;
+    const float* rows = qkv + (size_t)item * nodes * row_f + h * HD;
     const int s = streams[item], base = positions[item];
+    float2 x0[FRAGS][RH * PAIRS];
+#pragma unroll
+    for (int f = 0; f < FRAGS; f++)
+#pragma unroll
+        for (int i = 0; i < RH * PAIRS; i++) {
+            const int ks = (f * WARPS + warp) % QSTEPS, mt = (f * WARPS + warp) / QSTEPS;
+            const int t = t0 + mt * 16 + grp + (i % RH) * 8;
+            const int d = F32 ? (ks >> 1) * 16 + quad * 4 + (ks & 1) * 2 : ks * 16 + quad * 2 + (i / RH) * 8;
+            x0[f][i] = *reinterpret_cast<const float2*>(rows + (t < nodes ? t : 0) * row_f + d);
+        }
+    for (int i = tid; i < nodes * 4; i += 32 * WARPS)  // K, V: two lines each
+        prefetch_l2(rows + (i >> 2) * row_f + (size_t)(1 + ((i >> 1) & 1)) * H * HD + (i & 1) * 32);
     const bool in_range = s >= 0 && s < r.streams && base >= 0;
     const int window = in_range ? min(base, C) : 0;
     const int ring_tiles = (window + TS - 1) / TS, tree_tiles = (nodes + TS - 1) / TS;
@@ -222,6 +274,15 @@ __global__ void __launch_bounds__(32 * WARPS)
             }
         }
     };
+    // K and V of a tile into L2: PREFETCH tiles before they are copied, so that HBM stays busy while the block
+    // starts and joins
+    auto prefetch = [&](int tile) {
+        const int i = ring_tile(tile);
+        if (lane < 2 && i >= 0) {
+            const size_t row = plane + lane * (size_t)H * C + (size_t)i * TS;
+            bulk_prefetch_l2(reinterpret_cast<const T*>(r.kv) + row * HD, min(TS, window - i * TS) * HD * (int)sizeof(T));
+        }
+    };
     auto slot_position = [&](int tile) {
         const int j = ring_tile(tile) * TS + (lane & (TS - 1));
         return j >= 0 && j < window ? sp[j] : -1;
@@ -236,12 +297,15 @@ __global__ void __launch_bounds__(32 * WARPS)
     __syncwarp();
     if (ring_tile(tile) >= 0) fetch(tile, 0);
     if (ring_tile(tile + step) >= 0) fetch(tile + step, 1);
+#pragma unroll 1
+    for (int i = 2; i < 2 + PREFETCH; i++) prefetch(tile + i * step);
     if (warp == 0) tree_shape(sm.shape, parents + (size_t)item * nodes, nodes, lane);
     if (tid < NODES) sm.qmax[tid] = 0u;
+    if (tid < WARPS) sm.bad[tid] = 0u;
     __syncthreads();
 
     const TreeShape& sh = sm.shape;
-    const int max_depth = sh.max_depth, t0 = qt * NODES;
+    const int max_depth = sh.max_depth;
     const bool absent = !sh.bad && max_depth < 0;
     const int why = absent ? 0 : tree_reject(r, sh, s, base);
     if (absent || why) {
@@ -251,86 +315,60 @@ __global__ void __launch_bounds__(32 * WARPS)
         if (ring_tile(tile + step) >= 0) mbar_wait(&full[1], 0, WAIT_LIMIT);
         return;
     }
-    const size_t row_f = (size_t)3 * H * HD;
-    const float* rows = qkv + (size_t)item * nodes * row_f + h * HD;
 
-    // Builds a tile of the tree's own K and V, eight rows' loads at a time: lane i
-    // ropes dims (2 i, 2 i + 1).  Returns the nodes whose V is not finite.  (Absent
-    // nodes read row 0 and store zeros.)
-    auto build = [&](int tile, int st) -> uint32_t {
-        unsigned char* kd = stages + st * 2 * Tl::BYTES;
-        constexpr int PP = 16 / (2 * sizeof(T)), RB = 8;  // pairs per 16-byte piece, rows per batch
-        const int u0 = (tile - first) * TS;
-        uint32_t bad = 0u;
-#pragma unroll 1
-        for (int j0 = 0; j0 < TS && u0 + j0 < nodes; j0 += RB) {
-            float2 k[RB], v[RB], cs[RB];
-            uint32_t on = 0u;
+    // The tree's own K and V, RB rows of a tile by each warp of the block that holds the tile's owner: lane i ropes
+    // dims (2 i, 2 i + 1).  Absent nodes read row 0 and store zeros, as do the rows behind the last node: their
+    // weight is zero, and V has to be finite.
+    for (int u = 0; u < tree_tiles; u++) {
+        constexpr int PP = 16 / (2 * sizeof(T)), RB = TS / WARPS;  // pairs per 16-byte piece
+        const int at = first + u, owner = at % WARPS;
+        if (at % step / WARPS != rank) continue;
+        unsigned char* kd = sm.stage[owner][at / step];
+        float2 k[RB], v[RB], cs[RB];
+        uint32_t on = 0u, bad = 0u;
 #pragma unroll
-            for (int j = 0; j < RB; j++) {
-                const int u = u0 + j0 + j;
-                const unsigned long long path = u < nodes ? sh.path[u] : 0ull;
-                const float* src = rows + (path ? u : 0) * row_f;
-                const int pos = base + (path ? __popcll(path) - 1 : 0);
-                on |= path ? 1u << j : 0u;
-                k[j] = reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane];
-                v[j] = reinterpret_cast<const float2*>(src + (size_t)2 * H * HD)[lane];
-                cs[j] = r.rope[(size_t)pos * 32 + lane];
-            }
+        for (int j = 0; j < RB; j++) {
+            const int t = u * TS + warp * RB + j;
+            const unsigned long long path = t < nodes ? sh.path[t] : 0ull;
+            const float* src = rows + (path ? t : 0) * row_f;
+            on |= path ? 1u << j : 0u;
+            k[j] = reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane];
+            v[j] = reinterpret_cast<const float2*>(src + (size_t)2 * H * HD)[lane];
+            cs[j] = r.rope[(size_t)(base + (path ? __popcll(path) - 1 : 0)) * 32 + lane];
+        }
 #pragma unroll
-            for (int j = 0; j < RB; j++) {
-                const float2 kr = (on >> j) & 1u ? rope_pair(k[j], cs[j]) : make_float2(0.f, 0.f);
-                const float2 vr = (on >> j) & 1u ? v[j] : make_float2(0.f, 0.f);
-                alignas(8) const T kk[2] = {from_f<T>(kr.x), from_f<T>(kr.y)}, vv[2] = {from_f<T>(vr.x), from_f<T>(vr.y)};
-                const bool odd = !isfinite(to_f(vv[0])) || !isfinite(to_f(vv[1]));
-                if (__any_sync(0xffffffffu, odd)) bad |= 1u << (j0 + j);
-                T* ka = reinterpret_cast<T*>(kd + Tl::at(j0 + j, lane / PP)) + lane % PP * 2;
-                T* va = reinterpret_cast<T*>(kd + Tl::BYTES + Tl::at(j0 + j, lane / PP)) + lane % PP * 2;
-                if constexpr (F32) {
-                    *reinterpret_cast<float2*>(ka) = make_float2(kk[0], kk[1]);
-                    *reinterpret_cast<float2*>(va) = make_float2(vv[0], vv[1]);
-                } else {
-                    *reinterpret_cast<uint32_t*>(ka) = *reinterpret_cast<const uint32_t*>(kk);
-                    *reinterpret_cast<uint32_t*>(va) = *reinterpret_cast<const uint32_t*>(vv);
-                }
+        for (int j = 0; j < RB; j++) {
+            const float2 kr = (on >> j) & 1u ? rope_pair(k[j], cs[j]) : make_float2(0.f, 0.f);
+            const float2 vr = (on >> j) & 1u ? v[j] : make_float2(0.f, 0.f);
+            alignas(8) const T kk[2] = {from_f<T>(kr.x), from_f<T>(kr.y)}, vv[2] = {from_f<T>(vr.x), from_f<T>(vr.y)};
+            if (!isfinite(to_f(vv[0])) || !isfinite(to_f(vv[1]))) bad |= 1u << (warp * RB + j);
+            const int to = Tl::at(warp * RB + j, lane / PP) + lane % PP * 2 * (int)sizeof(T);
+            if constexpr (F32) {
+                *reinterpret_cast<float2*>(kd + to) = make_float2(kk[0], kk[1]);
+                *reinterpret_cast<float2*>(kd + Tl::BYTES + to) = make_float2(vv[0], vv[1]);
+            } else {
+                *reinterpret_cast<uint32_t*>(kd + to) = *reinterpret_cast<const uint32_t*>(kk);
+                *reinterpret_cast<uint32_t*>(kd + Tl::BYTES + to) = *reinterpret_cast<const uint32_t*>(vv);
             }
         }
-        // the rest of the tile: weight zero, so V has to be finite there
-        for (int j = max(0, (nodes - u0 + RB - 1) / RB * RB); j < TS; j++)
-            if (lane < HD * (int)sizeof(T) / 16)
-                *reinterpret_cast<uint4*>(kd + Tl::BYTES + Tl::at(j, lane)) = make_uint4(0u, 0u, 0u, 0u);
+        if (bad) atomicOr(&sm.bad[owner], bad);
         fence_async_smem();  // before a copy may write the stage
-        return bad;
-    };
+    }
 
-    // The block's rows of q: roped, scaled (f16), split, in the order the matrix
-    // instructions take them.  Pair i of a fragment is row grp (i even) or grp + 8,
-    // then, 16-bit, the pair of dims 8 further on.
+    // q: roped, scaled (f16), split
     {
-        constexpr int FRAGS = MT * QSTEPS / WARPS, PAIRS = F32 ? 1 : 2;  // pairs of a row
-        float2 x[FRAGS][RH * PAIRS], cs[FRAGS][RH * PAIRS];
-        bool on[FRAGS][RH * PAIRS];
-#pragma unroll
-        for (int f = 0; f < FRAGS; f++) {  // (every load before the first use; absent nodes read row 0)
-            const int ks = (f * WARPS + warp) % QSTEPS, mt = (f * WARPS + warp) / QSTEPS;
-#pragma unroll
-            for (int i = 0; i < RH * PAIRS; i++) {
-                const int t = t0 + mt * 16 + grp + (i % RH) * 8;
-                const int d = F32 ? (ks >> 1) * 16 + quad * 4 + (ks & 1) * 2 : ks * 16 + quad * 2 + (i / RH) * 8;
-                const unsigned long long path = t < nodes ? sh.path[t] : 0ull;
-                on[f][i] = path != 0ull;
-                x[f][i] = *reinterpret_cast<const float2*>(rows + (path ? t : 0) * row_f + d);
-                cs[f][i] = r.rope[(size_t)(base + (path ? __popcll(path) - 1 : 0)) * 32 + d / 2];
-            }
-        }
+        float2 x[FRAGS][RH * PAIRS];
 #pragma unroll
         for (int f = 0; f < FRAGS; f++)
 #pragma unroll
             for (int i = 0; i < RH * PAIRS; i++) {
-                x[f][i] = on[f][i] ? rope_pair(x[f][i], cs[f][i]) : make_float2(0.f, 0.f);
+                const int ks = (f * WARPS + warp) % QSTEPS, row = (f * WARPS + warp) / QSTEPS * 16 + grp + (i % RH) * 8;
+                const int d = F32 ? (ks >> 1) * 16 + quad * 4 + (ks & 1) * 2 : ks * 16 + quad * 2 + (i / RH) * 8;
+                const unsigned long long path = t0 + row < nodes ? sh.path[t0 + row] : 0ull;
+                const float2 cs = r.rope[(size_t)(base + (path ? __popcll(path) - 1 : 0)) * 32 + d / 2];
+                x[f][i] = path ? rope_pair(x0[f][i], cs) : make_float2(0.f, 0.f);
                 if constexpr (F16)
-                    atomicMax(&sm.qmax[(f * WARPS + warp) / QSTEPS * 16 + grp + (i % RH) * 8],
-                              __float_as_uint(fmaxf(fabsf(x[f][i].x), fabsf(x[f][i].y))));
+                    atomicMax(&sm.qmax[row], __float_as_uint(fmaxf(fabsf(x[f][i].x), fabsf(x[f][i].y))));
             }
         if constexpr (F16) __syncthreads();
         // f16: the row's largest |q| goes to [2^13, 2^14)
@@ -394,11 +432,6 @@ __global__ void __launch_bounds__(32 * WARPS)
         for (int i = 0; i < 8; i++)
 #pragma unroll
             for (int e = 0; e < 2 * RH; e++) o[mt][i][e] = 0.f;
-    uint32_t bad_cur = 0u, bad_next = 0u;
-    if (tile < tiles && ring_tile(tile) < 0) bad_cur = build(tile, 0);
-    if (tile + step < tiles && ring_tile(tile + step) < 0) bad_next = build(tile + step, 1);
-    __syncwarp();
-
     uint32_t phase = 0u;  // parity of the next copy into a stage, a bit each
     for (int st = 0; tile < tiles; tile += step, st ^= 1) {
         unsigned char* kd = stages + st * 2 * Tl::BYTES;
@@ -462,8 +495,8 @@ __global__ void __launch_bounds__(32 * WARPS)
                     const int row = i * 8 + (grp >> 1) + (grp & 1) * 4;
                     const float4 k = *reinterpret_cast<const float4*>(kd + Tl::at(row, j * 4 + quad));
                     uint32_t hi[4], lo[4];
-                    tf32_parts(k.x, hi[0], lo[0]), tf32_parts(k.y, hi[1], lo[1]);
-                    tf32_parts(k.z, hi[2], lo[2]), tf32_parts(k.w, hi[3], lo[3]);
+                    tf32_cut(k.x, hi[0], lo[0]), tf32_cut(k.y, hi[1], lo[1]);
+                    tf32_cut(k.z, hi[2], lo[2]), tf32_cut(k.w, hi[3], lo[3]);
 #pragma unroll
                     for (int e = 0; e < 2; e++)
 #pragma unroll
@@ -522,7 +555,7 @@ __global__ void __launch_bounds__(32 * WARPS)
                         if (!((see >> (8 * i + C1)) & 1u)) x[mt][i][2 * e + 1] = -INFINITY;
                     }
                 }
-            bad = bad_cur;
+            bad = sm.bad[warp];
         } else if (!__all_sync(0xffffffffu, seen >= max_depth)) {
 #pragma unroll
             for (int i = 0; i < NT; i++) {
@@ -645,14 +678,17 @@ __global__ void __launch_bounds__(32 * WARPS)
                         const float4 b =
                             *reinterpret_cast<const float4*>(kd + Tl::BYTES + Tl::at(i * 8 + quad + 4, 8 * c + pn));
                         const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+                        uint32_t h0[4], l0[4], h1[4], l1[4];
 #pragma unroll
-                        for (int f = 0; f < 4; f++) {
-                            uint32_t h0, l0, h1, l1;
-                            tf32_parts(av[f], h0, l0), tf32_parts(bv[f], h1, l1);
-                            if constexpr (!PACK) mma<T>(ot[4 * c + f], pl, h0, h1);
-                            mma<T>(ot[4 * c + f], ph, l0, l1);
-                            mma<T>(ot[4 * c + f], ph, h0, h1);
+                        for (int f = 0; f < 4; f++) tf32_cut(av[f], h0[f], l0[f]), tf32_cut(bv[f], h1[f], l1[f]);
+                        if constexpr (!PACK) {
+#pragma unroll
+                            for (int f = 0; f < 4; f++) mma<T>(ot[4 * c + f], pl, h0[f], h1[f]);
                         }
+#pragma unroll
+                        for (int f = 0; f < 4; f++) mma<T>(ot[4 * c + f], ph, l0[f], l1[f]);
+#pragma unroll
+                        for (int f = 0; f < 4; f++) mma<T>(ot[4 * c + f], ph, h0[f], h1[f]);
                     }
                 }
             } else {
@@ -667,17 +703,19 @@ __global__ void __launch_bounds__(32 * WARPS)
                             pair_parts<T>(x[mt][2 * i + f][2 * e], x[mt][2 * i + f][2 * e + 1], pp[RH * f + e]);
                         }
                     }
+                    uint32_t v[4][4];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {  // 16 dims
-                        uint32_t v[4];
-                        ldsm4t(v, vs + Tl::at(i * 16 + (lane & 15), 2 * c + (lane >> 4)));
+                    for (int c = 0; c < 4; c++)  // 16 dims
+                        ldsm4t(v[c], vs + Tl::at(i * 16 + (lane & 15), 2 * c + (lane >> 4)));
 #pragma unroll
-                        for (int p = Sm::QSETS - 1; p >= 0; p--) {
-                            const uint4 a =
-                                PACK ? make_uint4(pp[0][2 * p], pp[0][2 * p + 1], pp[1][2 * p], pp[1][2 * p + 1])
-                                     : make_uint4(pp[0][p], pp[1 % (RH * 2)][p], pp[2 % (RH * 2)][p], pp[3 % (RH * 2)][p]);
-                            mma<T>(ot[2 * c], a, v[0], v[1]);
-                            mma<T>(ot[2 * c + 1], a, v[2], v[3]);
+                    for (int p = Sm::QSETS - 1; p >= 0; p--) {
+                        const uint4 a =
+                            PACK ? make_uint4(pp[0][2 * p], pp[0][2 * p + 1], pp[1][2 * p], pp[1][2 * p + 1])
+                                 : make_uint4(pp[0][p], pp[1 % (RH * 2)][p], pp[2 % (RH * 2)][p], pp[3 % (RH * 2)][p]);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            mma<T>(ot[2 * c], a, v[c][0], v[c][1]);
+                            mma<T>(ot[2 * c + 1], a, v[c][2], v[c][3]);
                         }
                     }
                 }
@@ -689,10 +727,11 @@ __global__ void __launch_bounds__(32 * WARPS)
                     o[mt][i][e] = fmaf(o[mt][i][e], alpha[mt][e >> 1], PACK ? ot[i][e] + ot[i][e + 2 * (PACK ? 1 : 0)] : ot[i][e]);
         }
         __syncwarp();  // every lane is done with the stage
-        sp_cur = sp_next, bad_cur = bad_next, bad_next = 0u;
+        sp_cur = sp_next;
         const int ahead = tile + 2 * step;
         sp_next = slot_position(ahead);
         if (ring_tile(ahead) >= 0) fetch(ahead, st);
+        prefetch(ahead + PREFETCH * step);
     }
 
     // Join: each warp's rows to its own stages, then the warps' into the first.
@@ -896,7 +935,7 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
     attr.val.clusterDim = {(unsigned)splits, 1, 1};
     cfg.attrs = &attr;
     cfg.numAttrs = splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, map, r, nodes, qtiles, splits, streams, positions, parents, qkv, out);
+    return cudaLaunchKernelEx(&cfg, kernel, map, r, n, nodes, qtiles, splits, SORT, PFD, streams, positions, parents, qkv, out);
 }
 
 template <typename T>
