@@ -57,8 +57,6 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
                  : "memory");
 }
 
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
 // d[16 x 8] += a b with fp32 accumulation: bf16 or f16 operands 16 deep, tf32 operands 8 deep
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -155,16 +153,12 @@ __device__ __forceinline__ void pair_parts(float x, float y, uint32_t* p) {
 //
 // The rows of a matrix tile are 16 nodes, or (PACK, at most 8 nodes) two parts of
 // the same 8 nodes, whose products the lane that holds both adds up.
-constexpr int WARPS = 4, STAGES = 2, SORT_MAX = 256;
+constexpr int WARPS = 4, SORT_MAX = 256;
 #ifdef TUNE
 static int tune(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
 #define SPLIT_BELOW tune("SPLIT_BELOW", 296)
-#define PFD tune("PFD", 0)
-#define SORT (tune("SORT", 1) && n > 1 && n <= SORT_MAX)
-#define PREFETCH prefetch_dist
+#define SORT (tune("SORT", 1) && n > 1 && n <= SORT_MAX && blocks * splits > 2 * 148)
 #else
-#define PREFETCH 0
-#define PFD 0
 #define SORT (n > 1 && n <= SORT_MAX)
 #define SPLIT_BELOW 296
 #endif
@@ -184,28 +178,32 @@ struct Tile {
 
 template <typename T, int MT, bool PACK>
 struct alignas(1024) TreeSmem {
-    static constexpr int NODES = PACK ? 8 : 16 * MT;
+    static constexpr int NODES = PACK ? 8 : 16 * MT, STAGES = PACK ? 1 : 2;
     static constexpr int QSETS = sizeof(T) == 4 ? (PACK ? 1 : 2) : PACK ? (Parts<T>::N + 1) / 2 : Parts<T>::N;
     unsigned char stage[WARPS][STAGES][2 * Tile<T>::BYTES];  // K, then V
-    uint4 q[QSETS][MT][sizeof(T) == 4 ? 8 : 4][32];          // q as matrix operands: [part][tile][step][lane]
-    unsigned long long full[WARPS][STAGES], never;           // copies landed; never signalled (mb_set_wait_limit)
+    union {
+        uint4 q[QSETS][MT][sizeof(T) == 4 ? 8 : 4][32];      // q as matrix operands: [part][tile][step][lane]
+        int4 window[SORT_MAX / 4];                           // before that: of every item
+    };
+    unsigned long long full[WARPS][2], never;                // copies landed; never signalled (mb_set_wait_limit)
     float m[WARPS][NODES], l[WARPS][NODES];                  // [0]: the block's after the join
     float scale[NODES];                                      // of a score in units of log2
     unsigned int qmax[NODES];
     unsigned int bad[WARPS];                                 // nodes of the warp's tree tile whose V is not finite
     TreeShape shape;
-    int window[SORT_MAX], item;                              // of every item; the block's
+    int item;                                                // the block's (sort)
 };
 
 template <typename T, int MT, bool PACK>
 __global__ void __launch_bounds__(32 * WARPS)
-    tree_attend_kernel(const __grid_constant__ CUtensorMap map, RingView r, int n, int nodes, int qtiles, int splits, bool sort, int prefetch_dist,
+    tree_attend_kernel(const __grid_constant__ CUtensorMap map, RingView r, int n, int nodes, int qtiles, int splits, bool sort,
                        const int32_t* __restrict__ streams, const int32_t* __restrict__ positions,
                        const int32_t* __restrict__ parents, const float* __restrict__ qkv, float* __restrict__ out) {
     using Tl = Tile<T>;
     using Sm = TreeSmem<T, MT, PACK>;
     constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value;
     constexpr int TS = Tl::SLOTS, NT = TS / 8, NODES = Sm::NODES, QSTEPS = F32 ? 8 : 4, NP = Parts<T>::N;
+    constexpr int STAGES = Sm::STAGES;
     constexpr int RH = PACK ? 1 : 2;  // rows of a tile in one lane
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
@@ -218,27 +216,35 @@ __global__ void __launch_bounds__(32 * WARPS)
         // Blocks start in the order of their numbers, so the longest windows come first and the short ones fill
         // the gaps at the end: this block takes the item that `item` others come before.
         const int place = item;
-        for (int i = tid; i < n; i += 32 * WARPS) sm.window[i] = min(max(positions[i], 0), C);
+        int* window = &sm.window[0].x;
+        for (int i = tid; i < (n + 3) / 4 * 4; i += 32 * WARPS) window[i] = i < n ? min(max(positions[i], 0), C) : -1;
         __syncthreads();
         for (int i = tid; i < n; i += 32 * WARPS) {
-            const int w = sm.window[i];
+            const int w = window[i];
             int ahead = 0;
-            for (int j = 0; j < n; j++) ahead += sm.window[j] > w || (sm.window[j] == w && j < i);
+#pragma unroll 4
+            for (int j = 0; j < (n + 3) / 4; j++) {
+                const int4 v = sm.window[j];
+                ahead += (v.x > w || (v.x == w && 4 * j < i)) + (v.y > w || (v.y == w && 4 * j + 1 < i)) +
+                         (v.z > w || (v.z == w && 4 * j + 2 < i)) + (v.w > w || (v.w == w && 4 * j + 3 < i));
+            }
             if (ahead == place) sm.item = i;
         }
         __syncthreads();
         item = sm.item;
     }
 
-    // Everything that does not wait for the tree is on its way before the tree is looked at: the block's rows of q
+    // Everything that does not wait for the tree is asked for before the tree is looked at: the block's rows of q
     // (in the order the matrix instructions take them: pair i of a fragment is row grp (i even) or grp + 8, then,
-    // 16-bit, the pair of dims 8 further on), the tree's own K and V into L2, the ring's first tiles.
+    // 16-bit, the pair of dims 8 further on), the tree's K and V, the ring's first tiles.
     constexpr int FRAGS = MT * QSTEPS / WARPS, PAIRS = F32 ? 1 : 2;  // pairs of a row
+    constexpr int TREE = ((MT == 1 ? NODES : TREE_MAX_NODES) + TS - 1) / TS, RB = TS / WARPS;  // tree tiles; a warp's rows
     const int t0 = qt * NODES;
     const size_t row_f = (size_t)3 * H * HD;
     const float* rows = qkv + (size_t)item * nodes * row_f + h * HD;
+    const int2 parent = tree_parents(parents + (size_t)item * nodes, warp == 0 ? nodes : 0, lane);
     const int s = streams[item], base = positions[item];
-    float2 x0[FRAGS][RH * PAIRS];
+    float2 x0[FRAGS][RH * PAIRS], k0[TREE][RB], v0[TREE][RB];
 #pragma unroll
     for (int f = 0; f < FRAGS; f++)
 #pragma unroll
@@ -248,16 +254,24 @@ __global__ void __launch_bounds__(32 * WARPS)
             const int d = F32 ? (ks >> 1) * 16 + quad * 4 + (ks & 1) * 2 : ks * 16 + quad * 2 + (i / RH) * 8;
             x0[f][i] = *reinterpret_cast<const float2*>(rows + (t < nodes ? t : 0) * row_f + d);
         }
-    for (int i = tid; i < nodes * 4; i += 32 * WARPS)  // K, V: two lines each
-        prefetch_l2(rows + (i >> 2) * row_f + (size_t)(1 + ((i >> 1) & 1)) * H * HD + (i & 1) * 32);
+    if (rank == 0)
+#pragma unroll
+        for (int u = 0; u < TREE; u++)
+#pragma unroll
+            for (int j = 0; j < RB; j++) {
+                const int t = u * TS + warp * RB + j;
+                const float* src = rows + (t < nodes ? t : 0) * row_f;
+                k0[u][j] = reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane];
+                v0[u][j] = reinterpret_cast<const float2*>(src + (size_t)2 * H * HD)[lane];
+            }
     const bool in_range = s >= 0 && s < r.streams && base >= 0;
     const int window = in_range ? min(base, C) : 0;
     const int ring_tiles = (window + TS - 1) / TS, tree_tiles = (nodes + TS - 1) / TS;
     const int step = splits * WARPS;
-    // Warp w of the cluster takes tiles w, w + step, .. of: one ring tile for each warp, the tree's tiles (at most
-    // WARPS, so no warp builds one later than as its second), the ring's other tiles.
-    const int first = min(step, ring_tiles), tiles = ring_tiles + tree_tiles;
-    auto ring_tile = [&](int tile) { return tile < first ? tile : tile >= first + tree_tiles && tile < tiles ? tile - tree_tiles : -1; };
+    // Warp w of the cluster takes tiles w, w + step, ..: the tree's (at most WARPS: the first tiles of the first
+    // block's warps), then the ring's
+    const int tiles = tree_tiles + ring_tiles;
+    auto ring_tile = [&](int tile) { return tile < tiles ? tile - tree_tiles : -1; };  // negative: none
     const size_t plane = in_range ? ((size_t)s * 2 * H + h) * C : 0;  // K's rows in the map; V's lie H * C on
     const int32_t* sp = r.slot_pos + (in_range ? (size_t)s * C : 0);
     uint64_t* const full = reinterpret_cast<uint64_t*>(sm.full[warp]);
@@ -274,21 +288,12 @@ __global__ void __launch_bounds__(32 * WARPS)
             }
         }
     };
-    // K and V of a tile into L2: PREFETCH tiles before they are copied, so that HBM stays busy while the block
-    // starts and joins
-    auto prefetch = [&](int tile) {
-        const int i = ring_tile(tile);
-        if (lane < 2 && i >= 0) {
-            const size_t row = plane + lane * (size_t)H * C + (size_t)i * TS;
-            bulk_prefetch_l2(reinterpret_cast<const T*>(r.kv) + row * HD, min(TS, window - i * TS) * HD * (int)sizeof(T));
-        }
-    };
     auto slot_position = [&](int tile) {
         const int j = ring_tile(tile) * TS + (lane & (TS - 1));
         return j >= 0 && j < window ? sp[j] : -1;
     };
     int tile = rank * WARPS + warp;
-    int sp_cur = slot_position(tile), sp_next = slot_position(tile + step);
+    int sp_cur = slot_position(tile), sp_next = STAGES == 2 ? slot_position(tile + step) : -1;
     if (lane == 0) {
         mbar_init(&full[0], 1), mbar_init(&full[1], 1);
         if (warp == 0) mbar_init(reinterpret_cast<uint64_t*>(&sm.never), 1);
@@ -296,10 +301,8 @@ __global__ void __launch_bounds__(32 * WARPS)
     }
     __syncwarp();
     if (ring_tile(tile) >= 0) fetch(tile, 0);
-    if (ring_tile(tile + step) >= 0) fetch(tile + step, 1);
-#pragma unroll 1
-    for (int i = 2; i < 2 + PREFETCH; i++) prefetch(tile + i * step);
-    if (warp == 0) tree_shape(sm.shape, parents + (size_t)item * nodes, nodes, lane);
+    if (STAGES == 2 && ring_tile(tile + step) >= 0) fetch(tile + step, 1);
+    if (warp == 0) tree_shape(sm.shape, parent, nodes, lane);
     if (tid < NODES) sm.qmax[tid] = 0u;
     if (tid < WARPS) sm.bad[tid] = 0u;
     __syncthreads();
@@ -312,64 +315,72 @@ __global__ void __launch_bounds__(32 * WARPS)
         if (why && blockIdx.x % (splits * qtiles * H) == 0 && tid == 0) atomicOr(r.err, why);
         // no block leaves its shared memory while copies into it are under way
         if (ring_tile(tile) >= 0) mbar_wait(&full[0], 0, WAIT_LIMIT);
-        if (ring_tile(tile + step) >= 0) mbar_wait(&full[1], 0, WAIT_LIMIT);
+        if (STAGES == 2 && ring_tile(tile + step) >= 0) mbar_wait(&full[1], 0, WAIT_LIMIT);
         return;
     }
 
-    // The tree's own K and V, RB rows of a tile by each warp of the block that holds the tile's owner: lane i ropes
-    // dims (2 i, 2 i + 1).  Absent nodes read row 0 and store zeros, as do the rows behind the last node: their
-    // weight is zero, and V has to be finite.
-    for (int u = 0; u < tree_tiles; u++) {
-        constexpr int PP = 16 / (2 * sizeof(T)), RB = TS / WARPS;  // pairs per 16-byte piece
-        const int at = first + u, owner = at % WARPS;
-        if (at % step / WARPS != rank) continue;
-        unsigned char* kd = sm.stage[owner][at / step];
-        float2 k[RB], v[RB], cs[RB];
-        uint32_t on = 0u, bad = 0u;
-#pragma unroll
-        for (int j = 0; j < RB; j++) {
-            const int t = u * TS + warp * RB + j;
-            const unsigned long long path = t < nodes ? sh.path[t] : 0ull;
-            const float* src = rows + (path ? t : 0) * row_f;
-            on |= path ? 1u << j : 0u;
-            k[j] = reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane];
-            v[j] = reinterpret_cast<const float2*>(src + (size_t)2 * H * HD)[lane];
-            cs[j] = r.rope[(size_t)(base + (path ? __popcll(path) - 1 : 0)) * 32 + lane];
-        }
-#pragma unroll
-        for (int j = 0; j < RB; j++) {
-            const float2 kr = (on >> j) & 1u ? rope_pair(k[j], cs[j]) : make_float2(0.f, 0.f);
-            const float2 vr = (on >> j) & 1u ? v[j] : make_float2(0.f, 0.f);
-            alignas(8) const T kk[2] = {from_f<T>(kr.x), from_f<T>(kr.y)}, vv[2] = {from_f<T>(vr.x), from_f<T>(vr.y)};
-            if (!isfinite(to_f(vv[0])) || !isfinite(to_f(vv[1]))) bad |= 1u << (warp * RB + j);
-            const int to = Tl::at(warp * RB + j, lane / PP) + lane % PP * 2 * (int)sizeof(T);
-            if constexpr (F32) {
-                *reinterpret_cast<float2*>(kd + to) = make_float2(kk[0], kk[1]);
-                *reinterpret_cast<float2*>(kd + Tl::BYTES + to) = make_float2(vv[0], vv[1]);
-            } else {
-                *reinterpret_cast<uint32_t*>(kd + to) = *reinterpret_cast<const uint32_t*>(kk);
-                *reinterpret_cast<uint32_t*>(kd + Tl::BYTES + to) = *reinterpret_cast<const uint32_t*>(vv);
-            }
-        }
-        if (bad) atomicOr(&sm.bad[owner], bad);
-        fence_async_smem();  // before a copy may write the stage
-    }
-
-    // q: roped, scaled (f16), split
+    float2 x[FRAGS][RH * PAIRS];
     {
-        float2 x[FRAGS][RH * PAIRS];
+        // rope's factors, q's and K's loads together; absent nodes take the base's
+        float2 cs[FRAGS][RH * PAIRS], kcs[TREE][RB];
+        auto pos = [&](int t) {
+            const unsigned long long path = t < nodes ? sh.path[t] : 0ull;
+            return path ? __popcll(path) - 1 : -1;
+        };
 #pragma unroll
         for (int f = 0; f < FRAGS; f++)
 #pragma unroll
             for (int i = 0; i < RH * PAIRS; i++) {
                 const int ks = (f * WARPS + warp) % QSTEPS, row = (f * WARPS + warp) / QSTEPS * 16 + grp + (i % RH) * 8;
                 const int d = F32 ? (ks >> 1) * 16 + quad * 4 + (ks & 1) * 2 : ks * 16 + quad * 2 + (i / RH) * 8;
-                const unsigned long long path = t0 + row < nodes ? sh.path[t0 + row] : 0ull;
-                const float2 cs = r.rope[(size_t)(base + (path ? __popcll(path) - 1 : 0)) * 32 + d / 2];
-                x[f][i] = path ? rope_pair(x0[f][i], cs) : make_float2(0.f, 0.f);
+                cs[f][i] = r.rope[(size_t)(base + max(pos(t0 + row), 0)) * 32 + d / 2];
+            }
+        if (rank == 0) {
+#pragma unroll
+            for (int u = 0; u < TREE; u++)
+#pragma unroll
+                for (int j = 0; j < RB; j++)
+                    kcs[u][j] = r.rope[(size_t)(base + max(pos(u * TS + warp * RB + j), 0)) * 32 + lane];
+            // The tree's K and V: lane i has dims (2 i, 2 i + 1).  Absent nodes and the rows behind the last one
+            // become zeros: their weight is zero, and V has to be finite.
+#pragma unroll
+            for (int u = 0; u < TREE; u++) {
+                if (u >= tree_tiles) break;
+                constexpr int PP = 16 / (2 * sizeof(T));  // pairs per 16-byte piece
+                unsigned char* kd = sm.stage[u][0];
+                uint32_t bad = 0u;
+#pragma unroll
+                for (int j = 0; j < RB; j++) {
+                    const bool on = pos(u * TS + warp * RB + j) >= 0;
+                    const float2 kr = on ? rope_pair(k0[u][j], kcs[u][j]) : make_float2(0.f, 0.f);
+                    const float2 vr = on ? v0[u][j] : make_float2(0.f, 0.f);
+                    alignas(8) const T kk[2] = {from_f<T>(kr.x), from_f<T>(kr.y)}, vv[2] = {from_f<T>(vr.x), from_f<T>(vr.y)};
+                    if (!isfinite(to_f(vv[0])) || !isfinite(to_f(vv[1]))) bad |= 1u << (warp * RB + j);
+                    const int to = Tl::at(warp * RB + j, lane / PP) + lane % PP * 2 * (int)sizeof(T);
+                    if constexpr (F32) {
+                        *reinterpret_cast<float2*>(kd + to) = make_float2(kk[0], kk[1]);
+                        *reinterpret_cast<float2*>(kd + Tl::BYTES + to) = make_float2(vv[0], vv[1]);
+                    } else {
+                        *reinterpret_cast<uint32_t*>(kd + to) = *reinterpret_cast<const uint32_t*>(kk);
+                        *reinterpret_cast<uint32_t*>(kd + Tl::BYTES + to) = *reinterpret_cast<const uint32_t*>(vv);
+                    }
+                }
+                if (bad) atomicOr(&sm.bad[u], bad);
+            }
+            fence_async_smem();  // before a copy may write these stages
+        }
+#pragma unroll
+        for (int f = 0; f < FRAGS; f++)
+#pragma unroll
+            for (int i = 0; i < RH * PAIRS; i++) {
+                const int row = (f * WARPS + warp) / QSTEPS * 16 + grp + (i % RH) * 8;
+                x[f][i] = pos(t0 + row) >= 0 ? rope_pair(x0[f][i], cs[f][i]) : make_float2(0.f, 0.f);
                 if constexpr (F16)
                     atomicMax(&sm.qmax[row], __float_as_uint(fmaxf(fabsf(x[f][i].x), fabsf(x[f][i].y))));
             }
+    }
+    // q: scaled (f16), split
+    {
         if constexpr (F16) __syncthreads();
         // f16: the row's largest |q| goes to [2^13, 2^14)
         auto up = [&](int row) {
@@ -433,7 +444,7 @@ __global__ void __launch_bounds__(32 * WARPS)
 #pragma unroll
             for (int e = 0; e < 2 * RH; e++) o[mt][i][e] = 0.f;
     uint32_t phase = 0u;  // parity of the next copy into a stage, a bit each
-    for (int st = 0; tile < tiles; tile += step, st ^= 1) {
+    for (int st = 0; tile < tiles; tile += step, st ^= STAGES - 1) {
         unsigned char* kd = stages + st * 2 * Tl::BYTES;
         const uint32_t ks = smem_u32(kd), vs = ks + Tl::BYTES;
         const bool in_ring = ring_tile(tile) >= 0;
@@ -539,7 +550,7 @@ __global__ void __launch_bounds__(32 * WARPS)
         uint32_t bad = 0u;  // rows of V that are not finite and not seen by every node
         constexpr int C0 = F32 ? 1 : 2, C1 = F32 ? 4 : 1;  // a lane's columns: 8 i + C0 quad, and C1 further on
         if (!in_ring) {
-            const int u0 = (tile - first) * TS;
+            const int u0 = tile * TS;
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -727,11 +738,10 @@ __global__ void __launch_bounds__(32 * WARPS)
                     o[mt][i][e] = fmaf(o[mt][i][e], alpha[mt][e >> 1], PACK ? ot[i][e] + ot[i][e + 2 * (PACK ? 1 : 0)] : ot[i][e]);
         }
         __syncwarp();  // every lane is done with the stage
-        sp_cur = sp_next;
-        const int ahead = tile + 2 * step;
-        sp_next = slot_position(ahead);
+        const int ahead = tile + STAGES * step;
+        sp_cur = sp_next, sp_next = slot_position(ahead);
+        if (STAGES == 1) sp_cur = sp_next;
         if (ring_tile(ahead) >= 0) fetch(ahead, st);
-        prefetch(ahead + PREFETCH * step);
     }
 
     // Join: each warp's rows to its own stages, then the warps' into the first.
@@ -833,7 +843,8 @@ __global__ void __launch_bounds__(1024) tree_commit_kernel(RingView r, int n, in
                                                            int32_t* __restrict__ next_positions) {
     __shared__ TreeShape sh;
     const int H = r.heads, HID = H * HD, C = r.capacity, item = blockIdx.y, layer = blockIdx.z;
-    if (threadIdx.x < 32) tree_shape(sh, parents + (size_t)item * nodes, nodes, threadIdx.x);
+    if (threadIdx.x < 32)
+        tree_shape(sh, tree_parents(parents + (size_t)item * nodes, nodes, threadIdx.x), nodes, threadIdx.x);
     __syncthreads();
     const int s = streams[item], base = positions[item], leaf = leaves[item];
     const bool first = threadIdx.x == 0 && blockIdx.x == 0 && layer == 0;
@@ -935,7 +946,7 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
     attr.val.clusterDim = {(unsigned)splits, 1, 1};
     cfg.attrs = &attr;
     cfg.numAttrs = splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, map, r, n, nodes, qtiles, splits, SORT, PFD, streams, positions, parents, qkv, out);
+    return cudaLaunchKernelEx(&cfg, kernel, map, r, n, nodes, qtiles, splits, SORT, streams, positions, parents, qkv, out);
 }
 
 template <typename T>

@@ -13,57 +13,49 @@ constexpr int TREE_ABSENT = -2;
 // Topology of one item's tree in shared memory.
 struct TreeShape {
     unsigned long long path[TREE_MAX_NODES];  // bit u: u lies on the path root..t, t included; 0: absent
-    int link[TREE_MAX_NODES];                 // scratch of tree_shape
     int max_depth;                            // proper ancestors of the deepest node; -1: no node is present
     int bad;                                  // a parent that is neither -2, -1 nor an earlier present node
 };
 
-// Fills `sh` from parents[0, nodes), by one full warp (two nodes per lane).
-// Pointer doubling: after round i a node's mask holds its nearest 2^i ancestors
-// (itself included) and its link the node 2^i steps up, so log2(nodes) rounds
-// of one warp replace a walk of up to `nodes` dependent loads.  Reads only
-// indices checked against [0, t).
-__device__ __forceinline__ void tree_shape(TreeShape& sh, const int32_t* __restrict__ parents, int nodes, int lane) {
-    int par[2];
-    unsigned long long mask[2];
-    int link[2];
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-        const int t = lane + 32 * e;
-        par[e] = t < nodes ? parents[t] : TREE_ABSENT;
-        if (par[e] < TREE_ABSENT || par[e] >= t) {
-            if (t < nodes) bad = true;
-            par[e] = TREE_ABSENT;
-        }
-        mask[e] = par[e] == TREE_ABSENT ? 0ull : 1ull << t;
-        link[e] = par[e] < 0 ? -1 : par[e];
-        sh.path[t] = mask[e];
-        sh.link[t] = link[e];
-    }
-    __syncwarp();
-#pragma unroll
-    for (int e = 0; e < 2; e++)
-        if (link[e] >= 0 && sh.path[link[e]] == 0ull) bad = true;  // the parent is absent
+// Fills `sh` from par = (parents[lane], parents[lane + 32]) (tree_parents), by one
+// full warp.  Pointer doubling: after round i a node's mask holds its nearest 2^i
+// ancestors (itself included) and its link the node 2^i steps up, so log2(nodes)
+// rounds of one warp replace a walk of up to `nodes` dependent loads.  Follows
+// only links checked against [0, t).
+__device__ __forceinline__ int2 tree_parents(const int32_t* __restrict__ parents, int nodes, int lane) {
+    return make_int2(lane < nodes ? parents[lane] : TREE_ABSENT, lane + 32 < nodes ? parents[lane + 32] : TREE_ABSENT);
+}
+
+__device__ __forceinline__ void tree_shape(TreeShape& sh, int2 parent, int nodes, int lane) {
+    constexpr unsigned ALL = 0xffffffffu;
+    const bool bad0 = parent.x < TREE_ABSENT || parent.x >= lane, bad1 = parent.y < TREE_ABSENT || parent.y >= lane + 32;
+    const int par0 = bad0 ? TREE_ABSENT : parent.x, par1 = bad1 ? TREE_ABSENT : parent.y;
+    // nodes 0..31 descend from nodes below 32 alone
+    uint32_t low0 = par0 == TREE_ABSENT ? 0u : 1u << lane, low1 = 0u, high1 = par1 == TREE_ABSENT ? 0u : 1u << lane;
+    int link0 = par0 < 0 ? -1 : par0, link1 = par1 < 0 ? -1 : par1;
+    const uint32_t there0 = __ballot_sync(ALL, low0 != 0u), there1 = __ballot_sync(ALL, high1 != 0u);
+    bool bad = bad0 || bad1;  // or the parent is absent
+    if (link0 >= 0) bad |= !((there0 >> link0) & 1u);
+    if (link1 >= 0) bad |= !(((link1 < 32 ? there0 : there1) >> (link1 & 31)) & 1u);
     for (int span = 1; span < nodes; span <<= 1) {
-        unsigned long long m[2] = {0ull, 0ull};
-        int l[2] = {-1, -1};
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-            if (link[e] >= 0) m[e] = sh.path[link[e]], l[e] = sh.link[link[e]];
-        __syncwarp();
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            mask[e] |= m[e];
-            link[e] = l[e];
-            sh.path[lane + 32 * e] = mask[e];
-            sh.link[lane + 32 * e] = link[e];
+        const uint32_t a0 = __shfl_sync(ALL, low0, link0 & 31);
+        const int n0 = __shfl_sync(ALL, link0, link0 & 31);
+        if (nodes > 32) {
+            const uint32_t b0 = __shfl_sync(ALL, low0, link1 & 31), b1 = __shfl_sync(ALL, low1, link1 & 31);
+            const uint32_t b2 = __shfl_sync(ALL, high1, link1 & 31);
+            const int m0 = __shfl_sync(ALL, link0, link1 & 31), m1 = __shfl_sync(ALL, link1, link1 & 31);
+            if (link1 >= 32)
+                low1 |= b1, high1 |= b2, link1 = m1;
+            else if (link1 >= 0)
+                low1 |= b0, link1 = m0;
         }
-        __syncwarp();
+        if (link0 >= 0) low0 |= a0, link0 = n0;
     }
-    const int deep = max(__popcll(mask[0]), __popcll(mask[1])) - 1;
-    const int all_deep = __reduce_max_sync(0xffffffffu, deep);
-    const bool any_bad = __any_sync(0xffffffffu, bad);
+    sh.path[lane] = low0;
+    sh.path[lane + 32] = (unsigned long long)high1 << 32 | low1;
+    const int deep = max(__popc(low0), __popc(low1) + __popc(high1)) - 1;
+    const int all_deep = __reduce_max_sync(ALL, deep);
+    const bool any_bad = __any_sync(ALL, bad);
     if (lane == 0) sh.max_depth = all_deep, sh.bad = any_bad;
     __syncwarp();
 }
