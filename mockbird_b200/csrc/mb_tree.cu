@@ -16,9 +16,6 @@
 #include <cudaTypedefs.h>
 
 #include <atomic>
-#ifdef TUNE
-#include <stdlib.h>
-#endif
 #include <type_traits>
 
 #include "mb_ptx.cuh"
@@ -143,25 +140,22 @@ __device__ __forceinline__ void pair_parts(float x, float y, uint32_t* p) {
 //
 // A block takes NODES nodes of one item and head, over every `splits`-th group of
 // WARPS tiles of slots; the blocks of the other splits form its cluster.  Each warp
-// runs on its own: TMA brings its tiles of SLOTS slots (4 KB of K, 4 KB of V) into
-// its own two stages, and it keeps the running maximum, sum and context of its rows
-// in registers, so nothing in the loop waits for another warp.  The tree's own K
-// and V follow the ring's tiles as tiles of the same layout, built from the qkv
-// rows.  At the end the warps join through shared memory, then the blocks of the
-// cluster through distributed shared memory: no scratch in device memory, so calls
-// share nothing.
+// runs on its own: TMA brings a tile of SLOTS slots (4 KB of K, 4 KB of V) into its
+// own stage, and it keeps the running maximum, sum and context of its rows in
+// registers, so nothing in the loop waits for another warp; while one warp's tile
+// is on its way the SM's other warps compute (16 of them, 20 with PACK, 12 with two
+// matrix tiles of rows).  The tree's own K and V come first, as tiles of the same
+// layout, built from the qkv rows.  At the end the warps join through shared
+// memory, then the blocks of the cluster through distributed shared memory: no
+// scratch in device memory, so calls share nothing.
 //
 // The rows of a matrix tile are 16 nodes, or (PACK, at most 8 nodes) two parts of
 // the same 8 nodes, whose products the lane that holds both adds up.
-constexpr int WARPS = 4, SORT_MAX = 256;
-#ifdef TUNE
-static int tune(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-#define SPLIT_BELOW tune("SPLIT_BELOW", 296)
-#define SORT (tune("SORT", 1) && n > 1 && n <= SORT_MAX && blocks * splits > 2 * 148)
-#else
-#define SORT (n > 1 && n <= SORT_MAX)
-#define SPLIT_BELOW 296
-#endif
+//
+// mma.sync and not tcgen05: with 5 to 16 query rows per K and V row the 128 rows of
+// a tcgen05 tile would be almost empty.  The tensor pipe is 45 % busy where HBM
+// limits (16 nodes, bf16), and what limits 64 nodes.
+constexpr int WARPS = 4, SORT_MAX = 256, SMS = 148;
 
 template <typename T>
 struct Tile {
@@ -178,14 +172,14 @@ struct Tile {
 
 template <typename T, int MT, bool PACK>
 struct alignas(1024) TreeSmem {
-    static constexpr int NODES = PACK ? 8 : 16 * MT, STAGES = PACK ? 1 : 2;
+    static constexpr int NODES = PACK ? 8 : 16 * MT;
     static constexpr int QSETS = sizeof(T) == 4 ? (PACK ? 1 : 2) : PACK ? (Parts<T>::N + 1) / 2 : Parts<T>::N;
-    unsigned char stage[WARPS][STAGES][2 * Tile<T>::BYTES];  // K, then V
+    unsigned char stage[WARPS][2 * Tile<T>::BYTES];           // K, then V
     union {
         uint4 q[QSETS][MT][sizeof(T) == 4 ? 8 : 4][32];      // q as matrix operands: [part][tile][step][lane]
         int4 window[SORT_MAX / 4];                           // before that: of every item
     };
-    unsigned long long full[WARPS][2], never;                // copies landed; never signalled (mb_set_wait_limit)
+    unsigned long long full[WARPS], never;                   // copies landed; never signalled (mb_set_wait_limit)
     float m[WARPS][NODES], l[WARPS][NODES];                  // [0]: the block's after the join
     float scale[NODES];                                      // of a score in units of log2
     unsigned int qmax[NODES];
@@ -195,15 +189,14 @@ struct alignas(1024) TreeSmem {
 };
 
 template <typename T, int MT, bool PACK>
-__global__ void __launch_bounds__(32 * WARPS)
-    tree_attend_kernel(const __grid_constant__ CUtensorMap map, RingView r, int n, int nodes, int qtiles, int splits, bool sort,
-                       const int32_t* __restrict__ streams, const int32_t* __restrict__ positions,
+__global__ void __launch_bounds__(32 * WARPS, MT == 2 ? (sizeof(T) == 4 ? 2 : 3) : PACK ? 5 : 4)
+    tree_attend_kernel(const __grid_constant__ CUtensorMap map, RingView r, int n, int nodes, int qtiles, int splits,
+                       bool sort, const int32_t* __restrict__ streams, const int32_t* __restrict__ positions,
                        const int32_t* __restrict__ parents, const float* __restrict__ qkv, float* __restrict__ out) {
     using Tl = Tile<T>;
     using Sm = TreeSmem<T, MT, PACK>;
     constexpr bool F32 = sizeof(T) == 4, F16 = std::is_same<T, __half>::value;
     constexpr int TS = Tl::SLOTS, NT = TS / 8, NODES = Sm::NODES, QSTEPS = F32 ? 8 : 4, NP = Parts<T>::N;
-    constexpr int STAGES = Sm::STAGES;
     constexpr int RH = PACK ? 1 : 2;  // rows of a tile in one lane
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
@@ -274,17 +267,16 @@ __global__ void __launch_bounds__(32 * WARPS)
     auto ring_tile = [&](int tile) { return tile < tiles ? tile - tree_tiles : -1; };  // negative: none
     const size_t plane = in_range ? ((size_t)s * 2 * H + h) * C : 0;  // K's rows in the map; V's lie H * C on
     const int32_t* sp = r.slot_pos + (in_range ? (size_t)s * C : 0);
-    uint64_t* const full = reinterpret_cast<uint64_t*>(sm.full[warp]);
-    unsigned char* const stages = sm.stage[warp][0];
-    auto fetch = [&](int tile, int st) {
+    uint64_t* const full = reinterpret_cast<uint64_t*>(&sm.full[warp]);
+    unsigned char* const kd = sm.stage[warp];
+    auto fetch = [&](int tile) {
         if (lane == 0) {
-            unsigned char* kd = stages + st * 2 * Tl::BYTES;
             const int row = (int)plane + ring_tile(tile) * TS;
-            mbar_expect_tx(&full[st], 2 * Tl::BYTES);
+            mbar_expect_tx(full, 2 * Tl::BYTES);
 #pragma unroll
             for (int c = 0; c < Tl::BYTES / Tl::HALF; c++) {
-                tma_load_2d(kd + c * Tl::HALF, &map, c * 32, row, &full[st]);
-                tma_load_2d(kd + Tl::BYTES + c * Tl::HALF, &map, c * 32, row + H * C, &full[st]);
+                tma_load_2d(kd + c * Tl::HALF, &map, c * 32, row, full);
+                tma_load_2d(kd + Tl::BYTES + c * Tl::HALF, &map, c * 32, row + H * C, full);
             }
         }
     };
@@ -293,15 +285,14 @@ __global__ void __launch_bounds__(32 * WARPS)
         return j >= 0 && j < window ? sp[j] : -1;
     };
     int tile = rank * WARPS + warp;
-    int sp_cur = slot_position(tile), sp_next = STAGES == 2 ? slot_position(tile + step) : -1;
+    int sp_cur = slot_position(tile);
     if (lane == 0) {
-        mbar_init(&full[0], 1), mbar_init(&full[1], 1);
+        mbar_init(full, 1);
         if (warp == 0) mbar_init(reinterpret_cast<uint64_t*>(&sm.never), 1);
         fence_mbar_init();
     }
     __syncwarp();
-    if (ring_tile(tile) >= 0) fetch(tile, 0);
-    if (STAGES == 2 && ring_tile(tile + step) >= 0) fetch(tile + step, 1);
+    if (ring_tile(tile) >= 0) fetch(tile);
     if (warp == 0) tree_shape(sm.shape, parent, nodes, lane);
     if (tid < NODES) sm.qmax[tid] = 0u;
     if (tid < WARPS) sm.bad[tid] = 0u;
@@ -314,8 +305,7 @@ __global__ void __launch_bounds__(32 * WARPS)
     if (absent || why) {
         if (why && blockIdx.x % (splits * qtiles * H) == 0 && tid == 0) atomicOr(r.err, why);
         // no block leaves its shared memory while copies into it are under way
-        if (ring_tile(tile) >= 0) mbar_wait(&full[0], 0, WAIT_LIMIT);
-        if (STAGES == 2 && ring_tile(tile + step) >= 0) mbar_wait(&full[1], 0, WAIT_LIMIT);
+        if (ring_tile(tile) >= 0) mbar_wait(full, 0, WAIT_LIMIT);
         return;
     }
 
@@ -347,7 +337,7 @@ __global__ void __launch_bounds__(32 * WARPS)
             for (int u = 0; u < TREE; u++) {
                 if (u >= tree_tiles) break;
                 constexpr int PP = 16 / (2 * sizeof(T));  // pairs per 16-byte piece
-                unsigned char* kd = sm.stage[u][0];
+                unsigned char* kd = sm.stage[u];
                 uint32_t bad = 0u;
 #pragma unroll
                 for (int j = 0; j < RB; j++) {
@@ -443,21 +433,19 @@ __global__ void __launch_bounds__(32 * WARPS)
         for (int i = 0; i < 8; i++)
 #pragma unroll
             for (int e = 0; e < 2 * RH; e++) o[mt][i][e] = 0.f;
-    uint32_t phase = 0u;  // parity of the next copy into a stage, a bit each
-    for (int st = 0; tile < tiles; tile += step, st ^= STAGES - 1) {
-        unsigned char* kd = stages + st * 2 * Tl::BYTES;
-        const uint32_t ks = smem_u32(kd), vs = ks + Tl::BYTES;
+    const uint32_t ks = smem_u32(kd), vs = ks + Tl::BYTES;
+    for (uint32_t phase = 0u; tile < tiles; tile += step) {
         const bool in_ring = ring_tile(tile) >= 0;
         int seen = -1;  // this lane's slot is seen by nodes of depth <= seen
         bool landed = true;
         if (in_ring) {
-            uint64_t* bar = r.wait_probe ? reinterpret_cast<uint64_t*>(&sm.never) : &full[st];
-            landed = __all_sync(0xffffffffu, mbar_wait(bar, r.wait_probe ? 0u : (phase >> st) & 1u, r.wait_limit));
+            uint64_t* bar = r.wait_probe ? reinterpret_cast<uint64_t*>(&sm.never) : full;
+            landed = __all_sync(0xffffffffu, mbar_wait(bar, r.wait_probe ? 0u : phase, r.wait_limit));
             if (!landed) {  // the tile counts as empty, and its copies land before the stage is used again
                 if (lane == 0) atomicOr(r.err, DERR_TIMEOUT);
-                mbar_wait(&full[st], (phase >> st) & 1u, WAIT_LIMIT);
+                mbar_wait(full, phase, WAIT_LIMIT);
             }
-            phase ^= 1u << st;
+            phase ^= 1u;
             if (sp_cur >= 0 && sp_cur < base && landed) seen = C - 1 - (base - sp_cur);
             const uint32_t live = __ballot_sync(0xffffffffu, seen >= 0);
             if (live != ~0u) {  // slots that no node sees take part with weight zero: their V must be finite
@@ -665,87 +653,118 @@ __global__ void __launch_bounds__(32 * WARPS)
 
         // The context of this tile on its own, then one rounding into the running one: the tensor cores'
         // accumulation does not round to nearest, so its chains stay a tile long.
+        if constexpr (F32) {
+            uint4 ph[MT][NT], pl[MT][NT];  // 8 slots each
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            float ot[8][4];
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) ot[i][e] = 0.f;
-            if constexpr (F32) {
-#pragma unroll
-                for (int i = 0; i < NT; i++) {  // 8 slots
-                    uint4 ph, pl;
-                    tf32_parts(x[mt][i][0], ph.x, pl.x), tf32_parts(x[mt][i][1], ph.z, pl.z);
+                for (int i = 0; i < NT; i++) {
+                    uint4 &a = ph[mt][i], &b = pl[mt][i];
+                    tf32_parts(x[mt][i][0], a.x, b.x), tf32_parts(x[mt][i][1], a.z, b.z);
                     if constexpr (PACK)
-                        ph.y = pl.x, ph.w = pl.z;
+                        a.y = b.x, a.w = b.z;
                     else
-                        tf32_parts(x[mt][i][2], ph.y, pl.y), tf32_parts(x[mt][i][3], ph.w, pl.w);
-                    // column n of group 4 c + f is dim 32 c + 4 (n / 2 + 4 (n % 2)) + f
-                    const int pn = (grp >> 1) + (grp & 1) * 4;
+                        tf32_parts(x[mt][i][2], a.y, b.y), tf32_parts(x[mt][i][3], a.w, b.w);
+                }
+            // column n of group 4 c + f is dim 32 c + 4 (n / 2 + 4 (n % 2)) + f
+            const int pn = (grp >> 1) + (grp & 1) * 4;
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const float4 a = *reinterpret_cast<const float4*>(kd + Tl::BYTES + Tl::at(i * 8 + quad, 8 * c + pn));
-                        const float4 b =
-                            *reinterpret_cast<const float4*>(kd + Tl::BYTES + Tl::at(i * 8 + quad + 4, 8 * c + pn));
-                        const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-                        uint32_t h0[4], l0[4], h1[4], l1[4];
+            for (int c = 0; c < 2; c++) {
+                float ot[MT][4][4];
 #pragma unroll
-                        for (int f = 0; f < 4; f++) tf32_cut(av[f], h0[f], l0[f]), tf32_cut(bv[f], h1[f], l1[f]);
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int f = 0; f < 4; f++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) ot[mt][f][e] = 0.f;
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const float4 a = *reinterpret_cast<const float4*>(kd + Tl::BYTES + Tl::at(i * 8 + quad, 8 * c + pn));
+                    const float4 b =
+                        *reinterpret_cast<const float4*>(kd + Tl::BYTES + Tl::at(i * 8 + quad + 4, 8 * c + pn));
+                    const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+                    uint32_t h0[4], l0[4], h1[4], l1[4];
+#pragma unroll
+                    for (int f = 0; f < 4; f++) tf32_cut(av[f], h0[f], l0[f]), tf32_cut(bv[f], h1[f], l1[f]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
                         if constexpr (!PACK) {
 #pragma unroll
-                            for (int f = 0; f < 4; f++) mma<T>(ot[4 * c + f], pl, h0[f], h1[f]);
+                            for (int f = 0; f < 4; f++) mma<T>(ot[mt][f], pl[mt][i], h0[f], h1[f]);
                         }
 #pragma unroll
-                        for (int f = 0; f < 4; f++) mma<T>(ot[4 * c + f], ph, l0[f], l1[f]);
+                        for (int f = 0; f < 4; f++) mma<T>(ot[mt][f], ph[mt][i], l0[f], l1[f]);
 #pragma unroll
-                        for (int f = 0; f < 4; f++) mma<T>(ot[4 * c + f], ph, h0[f], h1[f]);
+                        for (int f = 0; f < 4; f++) mma<T>(ot[mt][f], ph[mt][i], h0[f], h1[f]);
                     }
                 }
-            } else {
 #pragma unroll
-                for (int i = 0; i < NT / 2; i++) {  // 16 slots
-                    uint32_t pp[RH * 2][NP + 1];
+                for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int f = 0; f < 2; f++) {
+                    for (int f = 0; f < 4; f++)
+#pragma unroll
+                        for (int e = 0; e < 2 * RH; e++)
+                            o[mt][4 * c + f][e] = fmaf(o[mt][4 * c + f][e], alpha[mt][e >> 1],
+                                                       PACK ? ot[mt][f][e] + ot[mt][f][(e + 2) & 3] : ot[mt][f][e]);
+            }
+        } else {
+            uint32_t pp[MT][NT / 2][RH * 2][NP + 1];  // 16 slots each
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int i = 0; i < NT / 2; i++)
+#pragma unroll
+                    for (int f = 0; f < 2; f++)
 #pragma unroll
                         for (int e = 0; e < RH; e++) {
-                            pp[RH * f + e][NP] = 0u;
-                            pair_parts<T>(x[mt][2 * i + f][2 * e], x[mt][2 * i + f][2 * e + 1], pp[RH * f + e]);
+                            pp[mt][i][RH * f + e][NP] = 0u;
+                            pair_parts<T>(x[mt][2 * i + f][2 * e], x[mt][2 * i + f][2 * e + 1], pp[mt][i][RH * f + e]);
                         }
-                    }
-                    uint32_t v[4][4];
 #pragma unroll
-                    for (int c = 0; c < 4; c++)  // 16 dims
-                        ldsm4t(v[c], vs + Tl::at(i * 16 + (lane & 15), 2 * c + (lane >> 4)));
+            for (int c = 0; c < 2; c++) {  // 32 dims at a time: few accumulators, and V read once for all rows
+                uint32_t v[NT / 2][2][4];
 #pragma unroll
-                    for (int p = Sm::QSETS - 1; p >= 0; p--) {
-                        const uint4 a =
-                            PACK ? make_uint4(pp[0][2 * p], pp[0][2 * p + 1], pp[1][2 * p], pp[1][2 * p + 1])
-                                 : make_uint4(pp[0][p], pp[1 % (RH * 2)][p], pp[2 % (RH * 2)][p], pp[3 % (RH * 2)][p]);
+                for (int i = 0; i < NT / 2; i++)
 #pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            mma<T>(ot[2 * c], a, v[c][0], v[c][1]);
-                            mma<T>(ot[2 * c + 1], a, v[c][2], v[c][3]);
+                    for (int d = 0; d < 2; d++)
+                        ldsm4t(v[i][d], vs + Tl::at(i * 16 + (lane & 15), 4 * c + 2 * d + (lane >> 4)));
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    float ot[4][4];
+#pragma unroll
+                    for (int f = 0; f < 4; f++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) ot[f][e] = 0.f;
+#pragma unroll
+                    for (int p = Sm::QSETS - 1; p >= 0; p--)
+#pragma unroll
+                        for (int i = 0; i < NT / 2; i++) {
+                            const uint32_t(&w)[RH * 2][NP + 1] = pp[mt][i];
+                            const uint4 a = PACK ? make_uint4(w[0][2 * p], w[0][2 * p + 1], w[1][2 * p], w[1][2 * p + 1])
+                                                 : make_uint4(w[0][p], w[1 % (RH * 2)][p], w[2 % (RH * 2)][p],
+                                                              w[3 % (RH * 2)][p]);
+#pragma unroll
+                            for (int d = 0; d < 2; d++) {
+                                mma<T>(ot[2 * d], a, v[i][d][0], v[i][d][1]);
+                                mma<T>(ot[2 * d + 1], a, v[i][d][2], v[i][d][3]);
+                            }
                         }
-                    }
+#pragma unroll
+                    for (int f = 0; f < 4; f++)
+#pragma unroll
+                        for (int e = 0; e < 2 * RH; e++)
+                            o[mt][4 * c + f][e] = fmaf(o[mt][4 * c + f][e], alpha[mt][e >> 1],
+                                                       PACK ? ot[f][e] + ot[f][(e + 2) & 3] : ot[f][e]);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-#pragma unroll
-                for (int e = 0; e < 2 * RH; e++)
-                    o[mt][i][e] = fmaf(o[mt][i][e], alpha[mt][e >> 1], PACK ? ot[i][e] + ot[i][e + 2 * (PACK ? 1 : 0)] : ot[i][e]);
         }
         __syncwarp();  // every lane is done with the stage
-        const int ahead = tile + STAGES * step;
-        sp_cur = sp_next, sp_next = slot_position(ahead);
-        if (STAGES == 1) sp_cur = sp_next;
-        if (ring_tile(ahead) >= 0) fetch(ahead, st);
+        sp_cur = slot_position(tile + step);
+        if (ring_tile(tile + step) >= 0) fetch(tile + step);
     }
 
-    // Join: each warp's rows to its own stages, then the warps' into the first.
-    float* mine = reinterpret_cast<float*>(stages);
+    // Join: each warp's rows to its own stage, then the warps' into the first.
+    float* mine = reinterpret_cast<float*>(kd);
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -784,7 +803,7 @@ __global__ void __launch_bounds__(32 * WARPS)
 #pragma unroll
         for (int w = 0; w < WARPS; w++) {
             const float a = ex2(sm.m[w][row] - use);
-            const float4 v = *reinterpret_cast<const float4*>(sm.stage[w][0] + (row * HD + d) * 4);
+            const float4 v = *reinterpret_cast<const float4*>(sm.stage[w] + (row * HD + d) * 4);
             acc.x = fmaf(a, v.x, acc.x), acc.y = fmaf(a, v.y, acc.y);
             acc.z = fmaf(a, v.z, acc.z), acc.w = fmaf(a, v.w, acc.w);
             sum = fmaf(a, sm.l[w][row], sum);
@@ -796,7 +815,7 @@ __global__ void __launch_bounds__(32 * WARPS)
                     make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             }
         } else {
-            *reinterpret_cast<float4*>(sm.stage[0][0] + (row * HD + d) * 4) = acc;
+            *reinterpret_cast<float4*>(sm.stage[0] + (row * HD + d) * 4) = acc;
             __syncwarp();  // the row's m and l are read by the 16 lanes of this half-warp before they are replaced
             if (d == 0) sm.m[0][row] = top, sm.l[0][row] = sum;
         }
@@ -815,7 +834,7 @@ __global__ void __launch_bounds__(32 * WARPS)
         float sum = 0.f;
         for (int b = 0; b < splits; b++) {
             const float a = ex2(*cluster.map_shared_rank(&sm.m[0][row], b) - use);
-            const float4 v = *cluster.map_shared_rank(reinterpret_cast<float4*>(sm.stage[0][0] + (row * HD + d) * 4), b);
+            const float4 v = *cluster.map_shared_rank(reinterpret_cast<float4*>(sm.stage[0] + (row * HD + d) * 4), b);
             acc.x = fmaf(a, v.x, acc.x), acc.y = fmaf(a, v.y, acc.y);
             acc.z = fmaf(a, v.z, acc.z), acc.w = fmaf(a, v.w, acc.w);
             sum = fmaf(a, *cluster.map_shared_rank(&sm.l[0][row], b), sum);
@@ -935,7 +954,8 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
     const int tiles = (r.capacity + Tile<T>::SLOTS - 1) / Tile<T>::SLOTS + (nodes + Tile<T>::SLOTS - 1) / Tile<T>::SLOTS;
     const int blocks = n * r.heads * qtiles;
     int splits = 1;
-    while (splits < 8 && blocks * splits < SPLIT_BELOW && splits * WARPS < tiles) splits *= 2;
+    while (splits < 8 && blocks * splits < 2 * SMS && splits * WARPS < tiles) splits *= 2;
+    const bool sort = n > 1 && n <= SORT_MAX && blocks * splits > 2 * SMS;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(blocks * splits);
     cfg.blockDim = dim3(32 * WARPS);
@@ -946,7 +966,7 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
     attr.val.clusterDim = {(unsigned)splits, 1, 1};
     cfg.attrs = &attr;
     cfg.numAttrs = splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, map, r, n, nodes, qtiles, splits, SORT, streams, positions, parents, qkv, out);
+    return cudaLaunchKernelEx(&cfg, kernel, map, r, n, nodes, qtiles, splits, sort, streams, positions, parents, qkv, out);
 }
 
 template <typename T>

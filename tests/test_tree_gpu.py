@@ -358,6 +358,49 @@ def test_capture_streams_and_determinism():
     assert all(torch.equal(x, wa) and torch.equal(y, wb) for x, y in got)
 
 
+def test_bounded_wait_runs_out_and_the_context_recovers():
+    """mb_set_wait_limit's probe: the waits for copies run out, the call returns, the next sync says so, and the
+    context goes on."""
+    H, C, T = 2, 300, 9
+    ring = KvRing(layers=1, heads=H, streams=2, capacity=C, dtype="f32", wrap=True, max_position=1024)
+    for s in range(2):
+        fill(ring, 0, s, 200, s)
+    trees = [tree_of("random", T, i) for i in range(2)]
+    qkv = normal((2, T, 3 * H * HD), 1)
+    want = ring.tree_attend(0, [0, 1], [200, 200], trees, qkv)
+    ring.sync()
+    ring.set_wait_limit(-20000)
+    ring.tree_attend(0, [0, 1], [200, 200], trees, qkv)
+    with pytest.raises(MockbirdError, match="TIMEOUT"):
+        ring.sync()
+    ring.set_wait_limit(0)
+    assert torch.equal(ring.tree_attend(0, [0, 1], [200, 200], trees, qkv), want)
+    ring.sync()
+
+
+@pytest.mark.parametrize("n,T,dtype", [(40, 16, "bf16"), (130, 5, "f32"), (70, 20, "f16")])
+def test_many_ragged_items(n, T, dtype):
+    """More blocks than run at once (their items are then taken longest window first), equal windows and empty
+    ones among them; every row against a call of its own."""
+    H, C = 12, 384
+    ring = KvRing(layers=1, heads=H, streams=n, capacity=C, dtype=dtype, wrap=True, max_position=2048)
+    r = random.Random(n)
+    bases = [r.choice([0, 7, 100, r.randrange(900)]) for _ in range(n)]
+    ids = list(range(n))
+    r.shuffle(ids)
+    for s, b in zip(ids, bases):
+        fill(ring, 0, s, b, s)
+    trees = [tree_of("random", T, i) for i in range(n)]
+    qkv = normal((n, T, 3 * H * HD), 5)
+    out = ring.tree_attend(0, ids, bases, trees, qkv)
+    for i in range(0, n, 3):
+        one = ring.tree_attend(0, ids[i:i + 1], bases[i:i + 1], trees[i:i + 1], qkv[i:i + 1])
+        # each side is within 1e-5 of the formula at unit inputs
+        assert (one[0] - out[i]).abs().max() < 2e-5, i
+    ring.sync()
+    check(ring, 0, ids[:4], bases[:4], trees[:4], qkv[:4], out[:4])
+
+
 def test_offsets_past_32_bits():
     """A stream whose rows start more than 2^31 elements (4 GB) into the ring."""
     H, C, S, T = 16, 1024, 1100, 9
