@@ -6,25 +6,21 @@
 #include <cooperative_groups.h>
 #include <limits.h>
 #include <math.h>
-#include <stdlib.h>
+
+#include <atomic>
 
 #include "mb_internal.cuh"
+#include "mb_ptx.cuh"
 
 namespace mb {
 
 namespace {
 
 constexpr int BEAM_MAX = 16;
-#ifndef FLIGHT
-#define FLIGHT 8
-#define BMIN 1
-#endif
-#ifdef TUNE
-static int tune(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-#define SEGMENT tune("SEGMENT", 256)
-#else
-constexpr int SEGMENT = 256;
-#endif
+// The split of a group over blocks (launch_select_t).  SEGMENT: 8 groups' worth of a 1024-code book take 21 us with
+// segments of 256 and more, 40 us with 64.  PLACES: 16 groups of 16 x 131071 take 43 us as clusters of 6 and 55 us as
+// clusters of 7 or 8, whose last ones share the SMs of others.
+constexpr int SEGMENT = 256, PLACES = 110;
 
 struct BeamArgs {
     int beams, codes, end_id;
@@ -59,11 +55,14 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// A double as an integer of the same order, so that a warp finds the largest of 32
-// with integer reductions (-0 counts as 0).
+// A double as an integer of the same order (-0 counts as 0), and back.
 __device__ __forceinline__ unsigned long long order_key(double v) {
     const long long k = __double_as_longlong(v + 0.0);
     return (unsigned long long)(k ^ ((k >> 63) & 0x7fffffffffffffffll)) ^ 0x8000000000000000ull;
+}
+__device__ __forceinline__ double key_value(unsigned long long key) {
+    const long long k = (long long)(key ^ 0x8000000000000000ull);
+    return __longlong_as_double(k ^ ((k >> 63) & 0x7fffffffffffffffll));
 }
 
 // ---------------------------------------------------------------- selection
@@ -76,37 +75,42 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
 //
 // The sum: exponentials in fp32 against a reference that the warp's maximum exceeds
 // by at most 8, batches of 16 added in fp32 and then in fp64.  An exponent x - ref
-// is off by at most 2^-23 of itself, whose mean under the softmax is at most
-// ln(codes) + 8 < 25, ex2 by 2^-22 and a batch's sum by 2^-22, so the log-sum-exp is
-// off by less than 3.5e-6 -- near the rounding of the returned score, but enough to
-// exchange two candidates of different beams that differ by less than 7e-6.  Such
-// neighbours (NEAR) at or above the last pick are rare; then the group's sums are taken again
-// in fp64, by the same warps, and the merge repeated, so the order is always that of
-// the values in 64 bits.  (All sums in fp64 would cost 14 fp64 operations per logit:
+// in units of log2 is off by at most 1.2 2^-23 of itself, whose mean under the
+// softmax is at most ln(codes) + 8 < 25, ex2 by 2^-22 and a batch's sum by 2^-22, so
+// the log-sum-exp is off by less than 3.9e-6 -- near the rounding of the returned
+// score, but enough to exchange two candidates of different beams that differ by
+// less than 7.8e-6.  Such neighbours (NEAR) at or above the last pick are rare; then
+// the group's sums are taken again in fp64, by the same warps, and the merge
+// repeated, so the order is always that of the values in 64 bits.  (All sums in fp64 would cost 14 fp64 operations per logit:
 // 1.4e12 logits/s on this part's fp64 units, against the 1.6e12 fp32 logits/s of HBM.)
 constexpr int BEAM_WARPS = 16, BEAM_CLUSTER = 8, UNITS = BEAM_WARPS * BEAM_CLUSTER;
-constexpr int CELLS = 12;  // per warp and lane
+constexpr int CELLS = 16, BEAM_STAGES = 2, POOL = 64;  // per warp (and lane)
 constexpr double NEAR = 8e-6;
 constexpr float ABOVE = 8.f;  // how far the warp's maximum may exceed its reference
 
+struct alignas(16) Candidate {
+    unsigned long long key;  // order_key of its value
+    int id, beam;            // beam * codes + code
+};
+
 struct BeamSmem {
-    float value[BEAM_WARPS][BEAM_MAX];  // a warp's list: logits, best first (-inf: none)
-    int id[BEAM_WARPS][BEAM_MAX];       // codes
-    double sum[BEAM_WARPS];             // of exp(x - top)
-    float top[BEAM_WARPS];              // the reference
-    float row_top[BEAM_MAX];
-    int again;
     union {
-        float cell[BEAM_WARPS][CELLS][32];  // the pass: largest values
-        struct {                            // the first block's merge
-            double cand[UNITS * BEAM_MAX];
-            int cand_id[UNITS * BEAM_MAX];
-        };
+        uint4 stage[BEAM_WARPS][BEAM_STAGES][128];  // the pass: batches on their way
+        Candidate cand[UNITS * BEAM_MAX];           // the first block's merge
     };
+    __nv_bfloat16 cell[BEAM_WARPS][CELLS][32];  // the pass: largest values, rounded up
+    // in the first block, written there by the warps of the whole cluster:
+    float value[UNITS][BEAM_MAX];  // a unit's list: logits, best first (-inf: none)
+    int id[UNITS][BEAM_MAX];       // codes
+    double sum[UNITS];             // of exp(x - top)
+    float top[UNITS];              // the reference
     double lse[BEAM_MAX];
-    int pick[BEAM_MAX];
+    float row_top[BEAM_MAX];
     float score[BEAM_MAX];
-    int done[BEAM_MAX];
+    int done[BEAM_MAX], pick[BEAM_MAX];
+    double pick_value[BEAM_MAX];
+    float head[UNITS], bound, row_need[BEAM_WARPS];
+    int count, again;
 };
 
 template <typename T, bool SEEN>
@@ -146,14 +150,18 @@ struct Segment {
     }
 };
 
+// A lane's own vectors of a batch to `dst` [VECS][32]: only this lane reads them.
 template <typename T>
-__device__ __forceinline__ void load_batch(const T* row, const Segment<T>& sg, int q, int l, uint4* raw) {
+__device__ __forceinline__ void fetch_batch(const T* row, const Segment<T>& sg, int q, int lane, uint4* dst) {
     const uint4* vp = reinterpret_cast<const uint4*>(row + sg.body);
 #pragma unroll
     for (int v = 0; v < Segment<T>::VECS; v++) {
-        const int at = l + 32 * (q * Segment<T>::VECS + v);
-        if (at < sg.nvec) raw[v] = vp[at];
+        const int at = lane + 32 * (q * Segment<T>::VECS + v);
+        if (at < sg.nvec)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + v * 32 + lane)), "l"(vp + at)
+                         : "memory");
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 // the batch's values, -inf behind the segment's last vector
@@ -176,8 +184,9 @@ __device__ __forceinline__ float tree_max(const float (&x)[N]) {
 }
 
 template <typename T, bool SEEN>
-__global__ void __launch_bounds__(32 * BEAM_WARPS, BMIN) beam_select_kernel(BeamArgs a, int blocks) {
-    __shared__ BeamSmem sm;
+__global__ void __launch_bounds__(32 * BEAM_WARPS, 2) beam_select_kernel(BeamArgs a, int blocks) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    BeamSmem& sm = *reinterpret_cast<BeamSmem*>(smem_raw);
     constexpr unsigned ALL = 0xffffffffu;
     namespace cg = cooperative_groups;
     const int B = a.beams, V = a.codes, g = blockIdx.x / blocks, rank = blockIdx.x % blocks;
@@ -192,6 +201,10 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, BMIN) beam_select_kernel(Beam
             __syncthreads();
     };
 
+    auto at_block = [&](auto* p, int r) {  // an object of the cluster's block r
+        return blocks > 1 ? cg::this_cluster().map_shared_rank(p, r) : p;
+    };
+    if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (waited for below)
     Row<T, SEEN> row{};
     bool live = false;
     if (unit < units) {
@@ -209,11 +222,13 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, BMIN) beam_select_kernel(Beam
     const Segment<T> sg(row.p, e0, e1);
     float top = -INFINITY;  // the warp's reference, and a lane's sum of exp(x - top)
     double sum = 0;
+    const int nb = live ? sg.batches() : 0, cell = (nb + CELLS - 1) / CELLS;
+    float lane_max = -INFINITY, edge = -INFINITY;
+    uint4* const stage = sm.stage[warp][0];
+    constexpr int VECS = Segment<T>::VECS;
     if (live) {
         // The pass: sums, and the largest value of every cell (CELL consecutive batches of a lane).
-        constexpr int VECS = Segment<T>::VECS, AHEAD = FLIGHT / VECS;  // batches in flight
-        const int nb = sg.batches(), cell = (nb + CELLS - 1) / CELLS;
-        float cell_max = -INFINITY, lane_max = -INFINITY;
+        float cell_max = -INFINITY;
         auto add = [&](auto& x, float m) {
             constexpr int N = sizeof(x) / sizeof(float);
             if (__any_sync(ALL, m > top + ABOVE)) {
@@ -232,118 +247,157 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, BMIN) beam_select_kernel(Beam
                 for (int e = 0; e < w; e++) s[e] += s[e + w];
             sum += (double)s[0];
         };
-        uint4 raw[AHEAD][VECS];
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) load_batch(row.p, sg, i, lane, raw[i]);
-        int in_cell = 0;
-        for (int q0 = 0; q0 < nb; q0 += AHEAD)
+        for (int i = 0; i < BEAM_STAGES; i++) fetch_batch(row.p, sg, i, lane, stage + i * 128);
+        for (int q = 0, st = 0, in_cell = 0; q < nb; q++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(BEAM_STAGES - 1) : "memory");
+            uint4 raw[VECS];
 #pragma unroll
-            for (int i = 0; i < AHEAD; i++) {
-                const int q = q0 + i;
-                if (q >= nb) break;
-                float x[16];
-                batch_values(row, sg, q, lane, raw[i], x);
-                load_batch(row.p, sg, q + AHEAD, lane, raw[i]);
-                const float m = tree_max(x);
-                add(x, m);
-                cell_max = fmaxf(cell_max, m);
-                if (++in_cell == cell || q == nb - 1) {
-                    sm.cell[warp][q / cell][lane] = cell_max;
-                    lane_max = fmaxf(lane_max, cell_max);
-                    cell_max = -INFINITY, in_cell = 0;
-                }
+            for (int v = 0; v < VECS; v++) raw[v] = stage[st * 128 + v * 32 + lane];
+            float x[16];
+            batch_values(row, sg, q, lane, raw, x);
+            fetch_batch(row.p, sg, q + BEAM_STAGES, lane, stage + st * 128);
+            st = st + 1 == BEAM_STAGES ? 0 : st + 1;
+            const float m = tree_max(x);
+            add(x, m);
+            cell_max = fmaxf(cell_max, m);
+            if (++in_cell == cell || q == nb - 1) {
+                sm.cell[warp][q / cell][lane] = __float2bfloat16_ru(cell_max);
+                lane_max = fmaxf(lane_max, cell_max);
+                cell_max = -INFINITY, in_cell = 0;
             }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         const int ej = sg.edge(lane);
-        float edge[1] = {ej >= 0 ? row.one(row.p[ej], ej) : -INFINITY};
-        add(edge, edge[0]);
+        float one[1] = {ej >= 0 ? row.one(row.p[ej], ej) : -INFINITY};
+        add(one, one[0]);
+        edge = one[0];
+    }
 
-        // The list, entry k in lane k.  At least `beams` values are no less than `need`, the beams-th largest of
-        // the lanes' maxima, and few more than that are: those in the cells that reach it, which are read again.
-        float lv = -INFINITY, need = -INFINITY;
-        int li = INT_MAX, need_id = INT_MAX, place = 0;
+    // A bound of what the row's best `beams` codes reach: at least `beams` values are no less than the beams-th
+    // largest of the lanes' maxima, and neither than the smallest, over the row's n warps in this block, of their
+    // ceil(beams / n)-th largest.
+    float need = -INFINITY;
+    float* const xs = reinterpret_cast<float*>(stage);            // a batch
+    float2* const pool = reinterpret_cast<float2*>(stage + 128);  // (value, code)
+    const int mates0 = max(b * segs - rank * BEAM_WARPS, 0), mates1 = min((b + 1) * segs - rank * BEAM_WARPS, BEAM_WARPS);
+    {
+        xs[lane] = lane_max;
+        __syncwarp();
+        int place = 0;
 #pragma unroll
-        for (int i = 0; i < 32; i++) place += before(__shfl_sync(ALL, lane_max, i), i, lane_max, lane);
-        const unsigned at = __ballot_sync(ALL, place == B - 1);
+        for (int i = 0; i < 8; i++) {
+            const float4 o = reinterpret_cast<const float4*>(xs)[i];
+            place += before(o.x, 4 * i, lane_max, lane) + before(o.y, 4 * i + 1, lane_max, lane) +
+                     before(o.z, 4 * i + 2, lane_max, lane) + before(o.w, 4 * i + 3, lane_max, lane);
+        }
+        const int n = max(mates1 - mates0, 1);
+        const unsigned at = __ballot_sync(ALL, place == B - 1), some = __ballot_sync(ALL, place == (B + n - 1) / n - 1);
         if (at) need = __shfl_sync(ALL, lane_max, __ffs(at) - 1);
-        auto insert = [&](auto& x, auto&& id) {
-            constexpr int N = sizeof(x) / sizeof(float);
-#pragma unroll
-            for (int e = 0; e < N; e++)
-                while (true) {
-                    const int j = id(e);
-                    const unsigned in = __ballot_sync(ALL, x[e] > -INFINITY && before(x[e], j, need, need_id));
-                    if (!in) break;
-                    const int src = __ffs(in) - 1;
-                    const float v = __shfl_sync(ALL, x[e], src);
-                    const int vj = __shfl_sync(ALL, j, src);
-                    if (lane == src) x[e] = -INFINITY;
-                    const int to = __popc(__ballot_sync(ALL, before(lv, li, v, vj)));
-                    const float uv = __shfl_up_sync(ALL, lv, 1);
-                    const int ui = __shfl_up_sync(ALL, li, 1);
-                    if (lane >= to) lv = lane == to ? v : uv, li = lane == to ? vj : ui;
-                    const float kv = __shfl_sync(ALL, lv, B - 1);
-                    const int ki = __shfl_sync(ALL, li, B - 1);
-                    if (kv > -INFINITY) need = kv, need_id = ki;
-                }
+        const float mine = some ? __shfl_sync(ALL, lane_max, __ffs(some) - 1) : -INFINITY;
+        if (lane == 0) sm.row_need[warp] = mine;
+    }
+    __syncthreads();
+    // every block of the cluster runs: the first one's shared memory may be written
+    if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (live) {
+        float together = INFINITY;
+        for (int w = mates0; w < mates1; w++) together = fminf(together, sm.row_need[w]);
+        need = fmaxf(need, together);
+        // The list: the values that reach the bound, which are read again where a cell says so, go to a pool, which
+        // is cut to the best `beams`, in order, when it is full and at the end.
+        int need_id = INT_MAX, pooled = 0;
+        auto cut = [&] {
+            __syncwarp();
+            const float2 none = make_float2(-INFINITY, __int_as_float(INT_MAX));
+            const float2 a = lane < pooled ? pool[lane] : none, c = lane + 32 < pooled ? pool[lane + 32] : none;
+            int ra = 0, rc = 0;
+#pragma unroll 4
+            for (int i = 0; i < pooled; i++) {
+                const float2 o = pool[i];
+                ra += before(o.x, __float_as_int(o.y), a.x, __float_as_int(a.y));
+                rc += before(o.x, __float_as_int(o.y), c.x, __float_as_int(c.y));
+            }
+            __syncwarp();
+            if (lane < pooled && ra < B) pool[ra] = a;
+            if (lane + 32 < pooled && rc < B) pool[rc] = c;
+            __syncwarp();
+            pooled = min(pooled, B);
+            if (pooled == B) need = pool[B - 1].x, need_id = __float_as_int(pool[B - 1].y);
         };
-        insert(edge, [&](int) { return ej; });
+        auto add_to_pool = [&](float x, int j, bool on) {  // one value of every lane that is `on`
+            on = on && x > -INFINITY && before(x, j, need, need_id);
+            unsigned in = __ballot_sync(ALL, on);
+            if (pooled + __popc(in) > POOL) {
+                cut();
+                on = on && before(x, j, need, need_id);
+                in = __ballot_sync(ALL, on);
+            }
+            if (on) pool[pooled + __popc(in & ((1u << lane) - 1u))] = make_float2(x, __int_as_float(j));
+            pooled += __popc(in);
+        };
+        if (sg.head | sg.tail) add_to_pool(edge, sg.edge(lane), edge > -INFINITY);
         // The cells that reach `need`, 32 at a time, one to a lane.
         const int used = nb ? (nb - 1) / cell + 1 : 0;
         int mine = -1, taken = 0;  // this lane's: cell * 32 + its lane
         auto flush = [&] {
             for (int g = 0; g < cell; g++) {
-                const int q = mine < 0 ? nb : (mine >> 5) * cell + g, l = mine & 31;
-                uint4 again[VECS];
-                float x[16];
-                load_batch(row.p, sg, q, l, again);
-                batch_values(row, sg, q, l, again, x);
-                if (q >= nb)
+                const int q = mine < 0 ? nb : min((mine >> 5) * cell + g, nb), l = mine & 31;  // nb: nothing
+                uint4 raw[VECS];
 #pragma unroll
-                    for (int e = 0; e < 16; e++) x[e] = -INFINITY;
-                if (__any_sync(ALL, tree_max(x) >= need)) insert(x, [&](int e) { return sg.code(q, l, e); });
+                for (int v = 0; v < VECS; v++) {
+                    const int at = l + 32 * (q * VECS + v);
+                    if (at < sg.nvec) raw[v] = reinterpret_cast<const uint4*>(row.p + sg.body)[at];
+                }
+                float x[16];
+                batch_values(row, sg, q, l, raw, x);
+                unsigned in = 0u;  // the lane's values that reach `need`, taken one by one through shared memory
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    xs[e * 32 + lane] = x[e];
+                    in |= x[e] >= need ? 1u << e : 0u;
+                }
+                while (__any_sync(ALL, in != 0u)) {
+                    const int e = in ? __ffs(in) - 1 : 0;
+                    add_to_pool(xs[e * 32 + lane], sg.code(q, l, e), in != 0u);
+                    in &= in - 1u;
+                }
             }
             mine = -1, taken = 0;
         };
         for (int k = 0; k < used; k++) {
-            const float c = sm.cell[warp][k][lane];
-            unsigned in = __ballot_sync(ALL, c >= need && c > -INFINITY);
-            while (in) {
-                const int fit = min(__popc(in), 32 - taken);
-                // the fit lowest lanes of `in` go to lanes taken .. taken + fit - 1
-                const int want = lane - taken;
-                const int src = want >= 0 && want < fit ? (int)__fns(in, 0, want + 1) : -1;
-                if (src >= 0) mine = k * 32 + src;
-                taken += fit;
-                for (int i = 0; i < fit; i++) in &= in - 1u;
-                if (taken == 32) flush();
+            const float c = __bfloat162float(sm.cell[warp][k][lane]);
+            for (unsigned in = __ballot_sync(ALL, c >= need && c > -INFINITY); in; in &= in - 1u) {
+                if (lane == taken) mine = k * 32 + __ffs(in) - 1;
+                if (++taken == 32) flush();
             }
         }
         if (taken) flush();
-        if (lane < B) sm.value[warp][lane] = lv, sm.id[warp][lane] = li;
-    } else if (lane < B) {
-        sm.value[warp][lane] = -INFINITY, sm.id[warp][lane] = INT_MAX;
+        cut();
+        if (lane < B) {
+            const float2 o = lane < pooled ? pool[lane] : make_float2(-INFINITY, __int_as_float(INT_MAX));
+            *at_block(&sm.value[unit][lane], 0) = o.x;
+            *at_block(&sm.id[unit][lane], 0) = __float_as_int(o.y);
+        }
+    } else if (lane == 0 && unit < units) {
+        *at_block(&sm.value[unit][0], 0) = -INFINITY;
     }
     auto put_sum = [&] {
         double s = sum;
         for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(ALL, s, i);
-        if (lane == 0) sm.top[warp] = top, sm.sum[warp] = s;
+        if (lane == 0 && unit < units) *at_block(&sm.top[unit], 0) = top, *at_block(&sm.sum[unit], 0) = s;
     };
     put_sum();
     sync();
 
-    // an object of the cluster's block r
-    auto at_block = [&](auto* p, int r) {
-        return blocks > 1 ? cg::this_cluster().map_shared_rank(p, r) : p;
-    };
     // The first block: every row's log-sum-exp, every candidate's value, the best `beams`.
     // Returns whether two of different beams, a pick and another, are too near to be told apart.
     auto merge = [&]() -> bool {
         for (int r = warp; r < B; r += BEAM_WARPS) {
             float m = -INFINITY, x = -INFINITY;  // the largest reference, the largest logit
             for (int i = lane; i < segs; i += 32) {
-                const int u = r * segs + i;
-                m = fmaxf(m, *at_block(&sm.top[u % BEAM_WARPS], u / BEAM_WARPS));
-                x = fmaxf(x, *at_block(&sm.value[u % BEAM_WARPS][0], u / BEAM_WARPS));
+                m = fmaxf(m, sm.top[r * segs + i]);
+                x = fmaxf(x, sm.value[r * segs + i][0]);
             }
             for (int i = 16; i > 0; i >>= 1) {
                 m = fmaxf(m, __shfl_xor_sync(ALL, m, i));
@@ -351,79 +405,73 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, BMIN) beam_select_kernel(Beam
             }
             double s = 0;
             for (int i = lane; i < segs; i += 32) {
-                const int u = r * segs + i;
-                const float t = *at_block(&sm.top[u % BEAM_WARPS], u / BEAM_WARPS);
-                const double p = *at_block(&sm.sum[u % BEAM_WARPS], u / BEAM_WARPS);
+                const float t = sm.top[r * segs + i];
+                const double p = sm.sum[r * segs + i];
                 s += t == -INFINITY ? p : p * exp((double)t - (double)m);
             }
             for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(ALL, s, i);
             if (lane == 0) sm.row_top[r] = x, sm.lse[r] = (double)m + log(s);
         }
         __syncthreads();
-        for (int i = tid; i < units * B; i += 32 * BEAM_WARPS) {
-            const int u = i / B, k = i % B, r = u / segs;
-            float x = *at_block(&sm.value[u % BEAM_WARPS][k], u / BEAM_WARPS);
-            int j = *at_block(&sm.id[u % BEAM_WARPS][k], u / BEAM_WARPS);
-            double v = (double)sm.score[r] + ((double)x - sm.lse[r]);
-            if (sm.done[r]) {  // goes on as it is, once
-                v = u % segs == 0 && k == 0 ? (double)sm.score[r] : -INFINITY;
-                j = a.end_id;
-            }
-            if (!isfinite((float)v)) v = -INFINITY;
-            sm.cand[u * B + k] = v;
-            sm.cand_id[u * B + k] = v > -INFINITY ? r * V + j : INT_MAX;
+        if (tid == 0) sm.count = 0, sm.bound = -INFINITY;
+        // the value of entry k of unit u's list; `at` its code
+        auto value = [&](int u, int k, int& at) -> double {
+            const int r = u / segs;
+            at = a.end_id;
+            if (sm.done[r]) return u % segs == 0 && k == 0 ? (double)sm.score[r] : -INFINITY;  // goes on as it is, once
+            at = sm.id[u][k];
+            const double v = (double)sm.score[r] + ((double)sm.value[u][k] - sm.lse[r]);
+            return isfinite((float)v) ? v : -INFINITY;
+        };
+        // The lists are sorted, so the beams-th best of their heads bounds the beams-th best of all from below.
+        // What reaches it, or comes so near that it may belong before the last pick, is sorted by counting.
+        int at = 0;
+        double v = -INFINITY;
+        if (tid < UNITS) {
+            if (tid < units) v = value(tid, 0, at);
+            sm.head[tid] = __double2float_rd(v);
         }
         __syncthreads();
+        if (tid < units) {
+            const float mine = sm.head[tid];
+            int ahead = 0;
+#pragma unroll 4
+            for (int u = 0; u < (units + 3) / 4; u++) {
+                const float4 o = reinterpret_cast<const float4*>(sm.head)[u];
+                ahead += before(o.x, 4 * u, mine, tid) + before(o.y, 4 * u + 1, mine, tid) +
+                         before(o.z, 4 * u + 2, mine, tid) + before(o.w, 4 * u + 3, mine, tid);
+            }
+            if (ahead == B - 1) sm.bound = mine;
+        }
+        if (tid < B) sm.pick[tid] = INT_MAX;
+        __syncthreads();
+        if (tid < units) {
+            const double bound = (double)sm.bound - NEAR;
+            for (int k = 0; v > -INFINITY && v >= bound;) {
+                const int r = tid / segs;
+                sm.cand[atomicAdd(&sm.count, 1)] = Candidate{order_key(v), r * V + at, r};
+                if (++k == B) break;
+                v = value(tid, k, at);
+            }
+        }
+        __syncthreads();
+        const int n = sm.count;
         bool near = false;
-        if (warp == 0) {
-            // lane l merges the lists of units l, l + 32, ..: sorted, so only their heads compete
-            constexpr int L = UNITS / 32;
-            double head[L];
-            int head_id[L], pos[L];
-#pragma unroll
-            for (int i = 0; i < L; i++) {
-                const int u = lane + 32 * i;
-                pos[i] = 0;
-                head[i] = u < units ? sm.cand[u * B] : -INFINITY;
-                head_id[i] = u < units ? sm.cand_id[u * B] : INT_MAX;
+        for (int i = tid; i < n; i += 32 * BEAM_WARPS) {
+            const Candidate c = sm.cand[i];
+            int ahead = 0;
+            unsigned long long next = 0;  // the best of another beam that is no better
+#pragma unroll 4
+            for (int k = 0; k < n; k++) {
+                const Candidate o = sm.cand[k];
+                const bool is = o.key > c.key || (o.key == c.key && o.id < c.id);
+                ahead += is;
+                if (!is && o.key > next && o.beam != c.beam) next = o.key;
             }
-            // Pick k in lane k; behind the last one, those so near to it that they may belong before it.
-            double pv = -INFINITY, least = -INFINITY;
-            int pi = INT_MAX, k = 0;
-            for (; k < 32; k++) {
-                double v = -INFINITY;
-                int id = INT_MAX, from = 0;
-#pragma unroll
-                for (int i = 0; i < L; i++)
-                    if (head[i] > v || (head[i] == v && head_id[i] < id)) v = head[i], id = head_id[i], from = i;
-                const unsigned long long key = order_key(v);
-                const unsigned hi = __reduce_max_sync(ALL, (unsigned)(key >> 32));
-                bool in = (unsigned)(key >> 32) == hi;
-                const unsigned lo = __reduce_max_sync(ALL, in ? (unsigned)key : 0u);
-                in = in && (unsigned)key == lo;
-                const int best = (int)__reduce_min_sync(ALL, in ? (unsigned)id : 0xffffffffu);
-                const int src = __ffs(__ballot_sync(ALL, in && id == best)) - 1;
-                const double bv = __shfl_sync(ALL, v, src);
-                if (bv == -INFINITY || (k >= B && least - bv >= NEAR)) break;
-                if (lane == k) pv = bv, pi = best;
-                if (k == B - 1) least = bv;
-                if (lane == src) {
-#pragma unroll
-                    for (int i = 0; i < L; i++)
-                        if (i == from) {
-                            const int u = lane + 32 * i;
-                            pos[i]++;
-                            head[i] = pos[i] < B ? sm.cand[u * B + pos[i]] : -INFINITY;
-                            head_id[i] = pos[i] < B ? sm.cand_id[u * B + pos[i]] : INT_MAX;
-                        }
-                }
-            }
-            const double nv = __shfl_down_sync(ALL, pv, 1);
-            const int ni = __shfl_down_sync(ALL, pi, 1);
-            near = k == 32 || __any_sync(ALL, lane < 31 && nv > -INFINITY && pv - nv < NEAR && pi / V != ni / V);
-            if (lane < B) {
-                sm.pick[lane] = pi;
-                sm.lse[lane] = pv;  // (the log-sum-exps are used up: the picks' values)
+            if (ahead < B) {
+                const double mine = key_value(c.key);
+                sm.pick[ahead] = c.id, sm.pick_value[ahead] = mine;
+                near |= next != 0 && mine - key_value(next) < NEAR;
             }
         }
         return __syncthreads_or(near);
@@ -458,7 +506,7 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, BMIN) beam_select_kernel(Beam
         const int from = there ? p / V : -1, j = there ? p % V : -1;
         a.parents[g * B + tid] = from;
         a.tokens[g * B + tid] = j;
-        a.scores_out[g * B + tid] = there ? (float)sm.lse[tid] : -INFINITY;
+        a.scores_out[g * B + tid] = there ? (float)sm.pick_value[tid] : -INFINITY;
         if (a.finished_out) a.finished_out[g * B + tid] = there ? (sm.done[from] || j == a.end_id) : sm.done[tid];
     }
     if constexpr (SEEN) {  // a thread carries one word of every row: all read before any is written
@@ -540,14 +588,31 @@ __global__ void __launch_bounds__(256) ring_reorder_kernel(RingView r, int beams
 
 template <typename T, bool SEEN>
 cudaError_t launch_select_t(int groups, const BeamArgs& a, cudaStream_t st) {
-    // blocks per group: enough for the SMs, a warp's segment no shorter than SEGMENT codes
+    // the opt-in to more than 48 KB of shared memory, once per device
+    static std::atomic<uint64_t> opted{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev > 63 || !(opted.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(beam_select_kernel<T, SEEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(BeamSmem));
+        if (e != cudaSuccess) return e;
+        opted.fetch_or(bit, std::memory_order_release);
+    }
+    // Blocks per group.  About PLACES blocks (clusters that stay within a GPC) find an SM of their own; what is
+    // above that waits or shares one, so the time goes with the rounds a group's blocks need over their number.
+    // A warp's segment is no shorter than SEGMENT codes.
     int blocks = 1;
-    while (blocks < BEAM_CLUSTER && groups * blocks < 2 * 148 &&
-           (long long)a.beams * a.codes >= 2ll * blocks * BEAM_WARPS * SEGMENT)
-        blocks *= 2;
+    for (int k = 2; k <= BEAM_CLUSTER; k++) {
+        if ((long long)a.beams * a.codes < (long long)k * BEAM_WARPS * SEGMENT) break;
+        const long long now = ((long long)groups * blocks + PLACES - 1) / PLACES;
+        const long long then = ((long long)groups * k + PLACES - 1) / PLACES;
+        if (then * blocks < now * k) blocks = k;
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(groups * blocks);
     cfg.blockDim = dim3(32 * BEAM_WARPS);
+    cfg.dynamicSmemBytes = sizeof(BeamSmem);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;

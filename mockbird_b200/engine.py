@@ -573,6 +573,12 @@ def argmax_penalty(logits: torch.Tensor, seen: torch.Tensor, penalty: float, str
 _DTYPE_CODE = {torch.float32: _lib.MB_F32, torch.bfloat16: _lib.MB_BF16, torch.float16: _lib.MB_F16}
 
 
+def _beam_array(name: str, t, dtype, shape, dev) -> None:
+    if not (isinstance(t, torch.Tensor) and t.device == dev and t.dtype is dtype and t.is_contiguous()
+            and t.shape == shape):
+        raise TypeError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {dev}")
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None = None, end_id: int = -1,
                 seen: torch.Tensor | None = None, penalty: float = 1.0, stream=None):
     """One beam-search step on the device: the best `beams` continuations of each group.
@@ -592,29 +598,29 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     row = logits.stride(1) if beams > 1 else logits.stride(0) if groups > 1 else codes
     if (codes > 1 and logits.stride(2) != 1) or (beams > 1 and groups > 1 and logits.stride(0) != beams * row):
         raise TypeError("logits' rows must be contiguous and evenly spaced")
-    dev = logits.device
-    for name, t, dtype, shape in (("scores", scores, torch.float32, (groups, beams)),
-                                  ("finished", finished, torch.int32, (groups, beams)),
-                                  ("seen", seen, torch.int32, (groups, beams, codes // 32))):
-        if t is None and name != "scores":
-            continue
-        if not (isinstance(t, torch.Tensor) and t.device == dev and t.dtype is dtype and t.is_contiguous()
-                and t.shape == shape):
-            raise TypeError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {dev}")
-    new = torch.empty(3 if finished is None else 4, groups, beams, dtype=torch.int32, device=dev)
+    dev, shape = logits.device, (groups, beams)
+    _beam_array("scores", scores, torch.float32, shape, dev)
+    new = torch.empty((3 if finished is None else 4, groups, beams), dtype=torch.int32, device=dev)
     _used_on(stream, new)
-    parents, tokens, out = new[0], new[1], new[2].view(torch.float32)
-    done = None if finished is None else new[3]
+    parents, tokens, out, *done = new.unbind()
+    out = out.view(torch.float32)
+    done = done[0] if done else None
+    if finished is not None:
+        _beam_array("finished", finished, torch.int32, shape, dev)
+    if seen is not None:
+        _beam_array("seen", seen, torch.int32, (groups, beams, codes // 32), dev)
     if stream is None:
         stream = _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
     elif isinstance(stream, torch.cuda.Stream):
         stream = stream.cuda_stream
-    with torch.cuda.device(dev):
-        rc = lib.mb_beam_select(groups, beams, codes, _DTYPE_CODE[logits.dtype], logits.data_ptr(), row,
-                                scores.data_ptr(), out.data_ptr(), None if finished is None else finished.data_ptr(),
-                                None if done is None else done.data_ptr(), end_id,
-                                None if seen is None else seen.data_ptr(), penalty, parents.data_ptr(),
-                                tokens.data_ptr(), int(stream))
+    args = (groups, beams, codes, _DTYPE_CODE[logits.dtype], logits.data_ptr(), row, scores.data_ptr(), out.data_ptr(),
+            None if finished is None else finished.data_ptr(), None if done is None else done.data_ptr(), end_id,
+            None if seen is None else seen.data_ptr(), penalty, parents.data_ptr(), tokens.data_ptr(), int(stream))
+    if dev.index == torch.cuda.current_device():
+        rc = lib.mb_beam_select(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = lib.mb_beam_select(*args)
     if rc:
         raise MockbirdError(rc, f"mb_beam_select: bad arguments or launch failure (groups={groups} beams={beams} "
                                 f"codes={codes} end_id={end_id} penalty={penalty})")
