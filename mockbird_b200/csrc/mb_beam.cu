@@ -21,6 +21,7 @@ constexpr int BEAM_MAX = 16;
 // segments of 256 and more, 40 us with 64.  PLACES: 16 groups of 16 x 131071 take 43 us as clusters of 6 and 55 us as
 // clusters of 7 or 8, whose last ones share the SMs of others.
 constexpr int SEGMENT = 256, PLACES = 110;
+constexpr int REORDER_BLOCKS = 4 * 148;
 
 struct BeamArgs {
     int beams, codes, end_id;
@@ -529,19 +530,23 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, 2) beam_select_kernel(BeamArg
 
 // ---------------------------------------------------------------- ring reorder
 
-// Stream k of a group takes the state of stream parents[k] of the group.  A
-// block owns REORDER_SLOTS slots of one layer and group, for K and V of every
-// head, so no other block touches what it reads or writes; a thread carries one
-// 16-byte piece of all the group's rows, and reads them all before it writes.
-constexpr int REORDER_SLOTS = 16;
-
-template <int B>
-__global__ void __launch_bounds__(256) ring_reorder_kernel(RingView r, int beams, int row16,
-                                                           const int32_t* __restrict__ streams,
-                                                           const int32_t* __restrict__ parents) {
-    __shared__ int s_stream[BEAM_MAX], s_from[BEAM_MAX], s_pos[BEAM_MAX][REORDER_SLOTS];
-    const int C = r.capacity, g = blockIdx.y, j0 = blockIdx.x * REORDER_SLOTS, tid = threadIdx.x;
-    char* kv = reinterpret_cast<char*>(r.kv) + (size_t)blockIdx.z * r.kv_layer * (row16 * 16 / HD);
+// Stream k of a group takes the state of stream parents[k] of the group.  A block
+// owns SLOTS slots of one layer and group, for K and V of every head, so no other
+// block touches what it reads or writes; a thread carries one 16-byte piece of all
+// the group's rows, and reads them all before it writes: in place, without a copy of
+// the state and whatever the cycles of the permutation.  (A group's beams share their
+// past, but which rows are equal cannot be known without reading both.)
+// Bound by HBM: 494 us for 8 groups of 8 beams on 1024-slot bf16 rings of 12 layers,
+// 3.1 GB at 6.3 TB/s (625 us without the streaming hints: what is read and written
+// here once would stay in L2 in place of what comes next); 26 us for one group of 4
+// on 570-slot fp32 rings (36 us with 16 slots to a block).
+template <int ROW16, int SLOTS, int B>  // 16-byte pieces of a row; beams <= B
+__global__ void __launch_bounds__(256) ring_reorder_kernel(RingView r, int beams,
+                                                                             const int32_t* __restrict__ streams,
+                                                                             const int32_t* __restrict__ parents) {
+    __shared__ int s_stream[B], s_from[B], s_pos[B][SLOTS];
+    const int C = r.capacity, g = blockIdx.y, j0 = blockIdx.x * SLOTS, tid = threadIdx.x;
+    const size_t stream16 = (size_t)2 * r.heads * C * ROW16;  // pieces of one stream and layer
     int32_t* slot_pos = r.slot_pos + (size_t)blockIdx.z * r.slot_layer;
     int why = 0;
     if (tid < beams) {
@@ -559,29 +564,29 @@ __global__ void __launch_bounds__(256) ring_reorder_kernel(RingView r, int beams
         if (why && blockIdx.x == 0 && blockIdx.z == 0) atomicOr(r.err, why);
         return;
     }
-    const int slots = min(REORDER_SLOTS, C - j0);
-    for (int i = tid; i < beams * REORDER_SLOTS; i += 256) {
-        const int k = i / REORDER_SLOTS, j = i % REORDER_SLOTS;
+    const int slots = min(SLOTS, C - j0);
+    for (int i = tid; i < beams * SLOTS; i += 256) {
+        const int k = i / SLOTS, j = i % SLOTS;
         s_pos[k][j] = j < slots ? slot_pos[(size_t)s_stream[k] * C + j0 + j] : -1;
     }
     __syncthreads();
-    const size_t stream16 = (size_t)2 * r.heads * C * row16;  // 16-byte pieces of one stream and layer
-    uint4* base = reinterpret_cast<uint4*>(kv);
-    const int per = slots * row16;
-    for (int i = tid; i < 2 * r.heads * per; i += 256) {
-        const int hv = i / per, x = i % per, j = x / row16;
-        const size_t at = ((size_t)hv * C + j0) * row16 + x;
+    uint4* kv = reinterpret_cast<uint4*>(r.kv) + (size_t)blockIdx.z * (r.kv_layer / HD) * ROW16;
+    constexpr int PER = SLOTS * ROW16;  // pieces of one head
+    const int pieces = 2 * r.heads * PER;
+    for (int i = tid; i < pieces; i += 256) {
+        const int j = i % PER / ROW16;
+        const size_t at = ((size_t)(i / PER) * C + j0) * ROW16 + i % PER;
         uint4 v[B];
 #pragma unroll
         for (int k = 0; k < B; k++)
             if (k < beams && s_from[k] != k && s_pos[s_from[k]][j] >= 0)
-                v[k] = base[s_stream[s_from[k]] * stream16 + at];
+                v[k] = __ldcs(kv + s_stream[s_from[k]] * stream16 + at);
 #pragma unroll
         for (int k = 0; k < B; k++)
-            if (k < beams && s_from[k] != k && s_pos[s_from[k]][j] >= 0) base[s_stream[k] * stream16 + at] = v[k];
+            if (k < beams && s_from[k] != k && s_pos[s_from[k]][j] >= 0) __stcs(kv + s_stream[k] * stream16 + at, v[k]);
     }
-    for (int i = tid; i < beams * REORDER_SLOTS; i += 256) {
-        const int k = i / REORDER_SLOTS, j = i % REORDER_SLOTS;
+    for (int i = tid; i < beams * SLOTS; i += 256) {
+        const int k = i / SLOTS, j = i % SLOTS;
         if (j < slots && s_from[k] != k) slot_pos[(size_t)s_stream[k] * C + j0 + j] = s_pos[s_from[k]][j];
     }
 }
@@ -639,17 +644,32 @@ bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) %
 
 }  // namespace
 
+namespace {
+
+template <int ROW16, int SLOTS>
+cudaError_t reorder_t(const RingView& r, int layers, int groups, int beams, const int32_t* streams,
+                      const int32_t* parents, cudaStream_t st) {
+    const dim3 grid((r.capacity + SLOTS - 1) / SLOTS, groups, layers);
+    if (beams <= 4)
+        ring_reorder_kernel<ROW16, SLOTS, 4><<<grid, 256, 0, st>>>(r, beams, streams, parents);
+    else if (beams <= 8)
+        ring_reorder_kernel<ROW16, SLOTS, 8><<<grid, 256, 0, st>>>(r, beams, streams, parents);
+    else
+        ring_reorder_kernel<ROW16, SLOTS, 16><<<grid, 256, 0, st>>>(r, beams, streams, parents);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
 cudaError_t launch_ring_reorder(int dtype, const RingView& r, int layers, int groups, int beams,
                                 const int32_t* streams, const int32_t* parents, cudaStream_t st) {
-    const int row16 = dtype == MB_F32 ? 16 : 8;
-    const dim3 grid((r.capacity + REORDER_SLOTS - 1) / REORDER_SLOTS, groups, layers);
-    if (beams <= 4)
-        ring_reorder_kernel<4><<<grid, 256, 0, st>>>(r, beams, row16, streams, parents);
-    else if (beams <= 8)
-        ring_reorder_kernel<8><<<grid, 256, 0, st>>>(r, beams, row16, streams, parents);
-    else
-        ring_reorder_kernel<16><<<grid, 256, 0, st>>>(r, beams, row16, streams, parents);
-    return cudaGetLastError();
+    // 16 slots to a block where that gives the SMs enough blocks (REORDER_BLOCKS), else 4
+    const bool wide = (long long)(r.capacity + 15) / 16 * groups * layers >= REORDER_BLOCKS;
+    if (dtype == MB_F32)
+        return wide ? reorder_t<16, 16>(r, layers, groups, beams, streams, parents, st)
+                    : reorder_t<16, 4>(r, layers, groups, beams, streams, parents, st);
+    return wide ? reorder_t<8, 16>(r, layers, groups, beams, streams, parents, st)
+                : reorder_t<8, 4>(r, layers, groups, beams, streams, parents, st);
 }
 
 }  // namespace mb

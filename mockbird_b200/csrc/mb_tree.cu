@@ -848,9 +848,14 @@ __global__ void __launch_bounds__(32 * WARPS, MT == 2 ? (sizeof(T) == 4 ? 2 : 3)
     cluster.sync();  // no block leaves while another reads its shared memory
 }
 
-// grid (node groups, items, layers), heads * 16 threads: each thread ropes and
-// stores four dims of one head, for the accepted nodes of its group.
-constexpr int COMMIT_NODES = 4;
+// ---------------------------------------------------------------- commit
+//
+// grid (COMMIT_BLOCKS at most, items, layers), heads * 16 threads: each thread
+// ropes and stores four dims of one head, for every gridDim.x-th node of the path.
+// 16.4 us for 64 streams of 12 layers with up to 16 accepted nodes, 56 MB (3.4 TB/s:
+// the wait for the tree in front of a few rows per block); 16.5 with 2 or 8 blocks,
+// 20 with one.
+constexpr int COMMIT_BLOCKS = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(1024) tree_commit_kernel(RingView r, int n, int nodes,
@@ -861,11 +866,12 @@ __global__ void __launch_bounds__(1024) tree_commit_kernel(RingView r, int n, in
                                                            const float* __restrict__ qkv,
                                                            int32_t* __restrict__ next_positions) {
     __shared__ TreeShape sh;
+    __shared__ unsigned char node[TREE_MAX_NODES];  // of the path, root first
     const int H = r.heads, HID = H * HD, C = r.capacity, item = blockIdx.y, layer = blockIdx.z;
+    const int s = streams[item], base = positions[item], leaf = leaves[item];
     if (threadIdx.x < 32)
         tree_shape(sh, tree_parents(parents + (size_t)item * nodes, nodes, threadIdx.x), nodes, threadIdx.x);
     __syncthreads();
-    const int s = streams[item], base = positions[item], leaf = leaves[item];
     const bool first = threadIdx.x == 0 && blockIdx.x == 0 && layer == 0;
     if (leaf == -1) {  // nothing accepted: the ring and the position stay
         if (first && next_positions) next_positions[item] = base;
@@ -880,31 +886,34 @@ __global__ void __launch_bounds__(1024) tree_commit_kernel(RingView r, int n, in
     const unsigned long long path = sh.path[leaf];
     const int len = __popcll(path);
     if (first && next_positions) next_positions[item] = base + len;
-    const int t0 = blockIdx.x * COMMIT_NODES, h = threadIdx.x >> 4, d4 = (threadIdx.x & 15) * 4;
-    T* kv = reinterpret_cast<T*>(r.kv) + (size_t)layer * r.kv_layer;
+    for (int t = threadIdx.x; t < nodes; t += blockDim.x)
+        if ((path >> t) & 1ull) node[__popcll(path & ((1ull << t) - 1ull))] = t;  // its ancestors come before it
+    __syncthreads();
+    const int h = threadIdx.x >> 4, d4 = (threadIdx.x & 15) * 4;
+    T* kd = reinterpret_cast<T*>(r.kv) + (size_t)layer * r.kv_layer + (((size_t)s * 2 + 0) * H + h) * C * HD + d4;
     int32_t* sp = r.slot_pos + (size_t)layer * r.slot_layer + (size_t)s * C;
-    for (int t = t0; t < min(t0 + COMMIT_NODES, nodes); t++) {
-        if (!((path >> t) & 1ull)) continue;
-        const int d = __popcll(path & ((1ull << t) - 1ull));  // t's proper ancestors: they come before it
-        if (len - d > C) continue;                            // the path's later nodes take this slot
-        const int pos = base + d, slot = pos % C;
-        const float* src = qkv + (((size_t)layer * n + item) * nodes + t) * 3 * HID + h * HD + d4;
-        const float4 k = *reinterpret_cast<const float4*>(src + HID), v = *reinterpret_cast<const float4*>(src + 2 * HID);
-        const float4 cs = *reinterpret_cast<const float4*>(r.rope + (size_t)pos * 32 + d4 / 2);
+    const float* rows = qkv + ((size_t)layer * n + item) * nodes * 3 * HID + h * HD + d4;
+    // (only the last C of the path: the earlier nodes' slots are theirs)
+    for (int d = max(len - C, 0) + blockIdx.x; d < len; d += gridDim.x) {
+        const float* src = rows + (size_t)node[d] * 3 * HID;
+        const float4 k = *reinterpret_cast<const float4*>(src + HID);
+        const float4 v = *reinterpret_cast<const float4*>(src + 2 * HID);
+        const float4 cs = *reinterpret_cast<const float4*>(r.rope + (size_t)(base + d) * 32 + d4 / 2);
         const float2 k0 = rope_pair(make_float2(k.x, k.y), make_float2(cs.x, cs.y));
         const float2 k1 = rope_pair(make_float2(k.z, k.w), make_float2(cs.z, cs.w));
-        T* kd = kv + ((((size_t)s * 2 + 0) * H + h) * C + slot) * HD + d4;
-        T* vd = kd + (size_t)H * C * HD;
-        alignas(16) T kq[4] = {from_f<T>(k0.x), from_f<T>(k0.y), from_f<T>(k1.x), from_f<T>(k1.y)};
-        alignas(16) T vq[4] = {from_f<T>(v.x), from_f<T>(v.y), from_f<T>(v.z), from_f<T>(v.w)};
+        alignas(16) const T kq[4] = {from_f<T>(k0.x), from_f<T>(k0.y), from_f<T>(k1.x), from_f<T>(k1.y)};
+        alignas(16) const T vq[4] = {from_f<T>(v.x), from_f<T>(v.y), from_f<T>(v.z), from_f<T>(v.w)};
+        const int slot = (base + d) % C;
+        T* to = kd + (size_t)slot * HD;
+        T* vto = to + (size_t)H * C * HD;
         if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(kd) = *reinterpret_cast<const float4*>(kq);
-            *reinterpret_cast<float4*>(vd) = *reinterpret_cast<const float4*>(vq);
+            *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(kq);
+            *reinterpret_cast<float4*>(vto) = *reinterpret_cast<const float4*>(vq);
         } else {
-            *reinterpret_cast<uint2*>(kd) = *reinterpret_cast<const uint2*>(kq);
-            *reinterpret_cast<uint2*>(vd) = *reinterpret_cast<const uint2*>(vq);
+            *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(kq);
+            *reinterpret_cast<uint2*>(vto) = *reinterpret_cast<const uint2*>(vq);
         }
-        if (threadIdx.x == 0) sp[slot] = pos;
+        if (threadIdx.x == 0) sp[slot] = base + d;
     }
 }
 
@@ -981,7 +990,7 @@ template <typename T>
 cudaError_t commit_t(const RingView& r, int layers, int n, int nodes, const int32_t* streams,
                      const int32_t* positions, const int32_t* parents, const int32_t* leaves, const float* qkv,
                      int32_t* next_positions, cudaStream_t st) {
-    const dim3 grid((nodes + COMMIT_NODES - 1) / COMMIT_NODES, n, layers);
+    const dim3 grid(nodes < COMMIT_BLOCKS ? nodes : COMMIT_BLOCKS, n, layers);
     tree_commit_kernel<T><<<grid, r.heads * 16, 0, st>>>(r, n, nodes, streams, positions, parents, leaves, qkv,
                                                          next_positions);
     return cudaGetLastError();
