@@ -419,7 +419,8 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, 2) beam_select_kernel(BeamArg
         auto value = [&](int u, int k, int& at) -> double {
             const int r = u / segs;
             at = a.end_id;
-            if (sm.done[r]) return u % segs == 0 && k == 0 ? (double)sm.score[r] : -INFINITY;  // goes on as it is, once
+            if (sm.done[r])  // goes on as it is, once
+                return u % segs == 0 && k == 0 && isfinite(sm.score[r]) ? (double)sm.score[r] : -INFINITY;
             at = sm.id[u][k];
             const double v = (double)sm.score[r] + ((double)sm.value[u][k] - sm.lse[r]);
             return isfinite((float)v) ? v : -INFINITY;
@@ -600,7 +601,8 @@ cudaError_t launch_select_t(int groups, const BeamArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
     if (dev > 63 || !(opted.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(beam_select_kernel<T, SEEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(BeamSmem));
+        e = cudaFuncSetAttribute(beam_select_kernel<T, SEEN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 sizeof(BeamSmem));
         if (e != cudaSuccess) return e;
         opted.fetch_or(bit, std::memory_order_release);
     }
@@ -624,7 +626,9 @@ cudaError_t launch_select_t(int groups, const BeamArgs& a, cudaStream_t st) {
     attr.val.clusterDim = {(unsigned)blocks, 1, 1};
     cfg.attrs = &attr;
     cfg.numAttrs = blocks > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, beam_select_kernel<T, SEEN>, a, blocks);
+    e = cudaLaunchKernelEx(&cfg, beam_select_kernel<T, SEEN>, a, blocks);
+    if (e != cudaSuccess) cudaGetLastError();  // reported here, not by the next launch
+    return e;
 }
 
 template <typename T>

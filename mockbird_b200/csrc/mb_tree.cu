@@ -850,8 +850,9 @@ __global__ void __launch_bounds__(32 * WARPS, MT == 2 ? (sizeof(T) == 4 ? 2 : 3)
 
 // ---------------------------------------------------------------- commit
 //
-// grid (COMMIT_BLOCKS at most, items, layers), heads * 16 threads: each thread
-// ropes and stores four dims of one head, for every gridDim.x-th node of the path.
+// grid (COMMIT_BLOCKS at most, items, layers), heads * 16 threads (a full warp at
+// least, for the tree): each ropes and stores four dims of one head, for every
+// gridDim.x-th node of the path.
 // 16.4 us for 64 streams of 12 layers with up to 16 accepted nodes, 56 MB (3.4 TB/s:
 // the wait for the tree in front of a few rows per block); 16.5 with 2 or 8 blocks,
 // 20 with one.
@@ -890,6 +891,7 @@ __global__ void __launch_bounds__(1024) tree_commit_kernel(RingView r, int n, in
         if ((path >> t) & 1ull) node[__popcll(path & ((1ull << t) - 1ull))] = t;  // its ancestors come before it
     __syncthreads();
     const int h = threadIdx.x >> 4, d4 = (threadIdx.x & 15) * 4;
+    if (h >= H) return;
     T* kd = reinterpret_cast<T*>(r.kv) + (size_t)layer * r.kv_layer + (((size_t)s * 2 + 0) * H + h) * C * HD + d4;
     int32_t* sp = r.slot_pos + (size_t)layer * r.slot_layer + (size_t)s * C;
     const float* rows = qkv + ((size_t)layer * n + item) * nodes * 3 * HID + h * HD + d4;
@@ -975,7 +977,9 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
     attr.val.clusterDim = {(unsigned)splits, 1, 1};
     cfg.attrs = &attr;
     cfg.numAttrs = splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, map, r, n, nodes, qtiles, splits, sort, streams, positions, parents, qkv, out);
+    e = cudaLaunchKernelEx(&cfg, kernel, map, r, n, nodes, qtiles, splits, sort, streams, positions, parents, qkv, out);
+    if (e != cudaSuccess) cudaGetLastError();  // reported here, not by the next launch
+    return e;
 }
 
 template <typename T>
@@ -991,7 +995,7 @@ cudaError_t commit_t(const RingView& r, int layers, int n, int nodes, const int3
                      const int32_t* positions, const int32_t* parents, const int32_t* leaves, const float* qkv,
                      int32_t* next_positions, cudaStream_t st) {
     const dim3 grid(nodes < COMMIT_BLOCKS ? nodes : COMMIT_BLOCKS, n, layers);
-    tree_commit_kernel<T><<<grid, r.heads * 16, 0, st>>>(r, n, nodes, streams, positions, parents, leaves, qkv,
+    tree_commit_kernel<T><<<grid, r.heads < 2 ? 32 : r.heads * 16, 0, st>>>(r, n, nodes, streams, positions, parents, leaves, qkv,
                                                          next_positions);
     return cudaGetLastError();
 }

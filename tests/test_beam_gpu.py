@@ -94,6 +94,29 @@ def test_one_beam_is_the_greedy_argmax():
     assert torch.equal(t.flatten(), want) and torch.equal(seen.view(n, -1), other) and (p == 0).all() and d is None
 
 
+def test_rows_past_32_bits():
+    """Rows that start more than 2^31 elements behind the first."""
+    G, B, V, stride = 5, 7, 700, 1 << 26
+    flat = torch.empty(G * B * stride, device=DEV, dtype=torch.bfloat16)
+    rows = flat.view(G, B, stride)[:, :, :V]
+    rows.copy_(normal((G, B, V), 8, 3.0))
+    check(rows, -normal((G, B), 9).abs())
+
+
+@pytest.mark.parametrize("where", ["rising", "falling", "last", "first"])
+def test_where_the_largest_stand(where):
+    """Rows sorted either way (the reference of the sum moves, every batch beats the last) and rows whose largest
+    codes stand in the first or last few places."""
+    G, B, V = 2, 9, 70001
+    rows, scores = case(G, B, V, "f32", 4, 3, 1)
+    if where in ("rising", "falling"):
+        rows.copy_(rows.sort(-1, descending=where == "falling").values * 20)
+    else:
+        at = slice(V - 12, V) if where == "last" else slice(0, 12)
+        rows[:, :, at] += 60
+    check(rows, scores)
+
+
 def test_ties_go_to_the_lowest_index():
     G, B, V = 4, 5, 1500
     rows = torch.zeros(G, B, V, device=DEV)
@@ -125,6 +148,9 @@ def test_nothing_to_propose():
     finished[:, 0] = 1
     finished[1] = 1
     scores[1, 2] = -INF
+    check(rows, scores, finished, 17)
+    finished[6] = 1                    # finished hypotheses with scores that are none
+    finished[5, 1] = 1
     check(rows, scores, finished, 17)
     seen = masks((G, B, 19), 31)
     check(rows[:, :, :576], scores, finished, 17, seen[:, :, :18].contiguous(), 1.3)

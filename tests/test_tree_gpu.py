@@ -1,6 +1,7 @@
 """Attention of a tree of drafted tokens over the ring, and the commit of an accepted path, against the plain
 64-bit form (search_util) and against append_attend one node after another."""
 import ctypes
+import os
 import random
 
 import numpy as np
@@ -116,10 +117,11 @@ def test_tree_against_64_bits(dtype, T, C, bases, wrap, kind):
     assert torch.equal(held.slot_pos, sp) and torch.equal(held.kv, kv)  # the rings are only read
 
 
+@pytest.mark.parametrize("T", [5, 9, 33])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-def test_large_scores_and_skewed_rows(dtype):
+def test_large_scores_and_skewed_rows(dtype, T):
     """Scores of some hundreds (one slot takes the whole weight) and rows of very different size."""
-    H, C, T = 2, 257, 9
+    H, C = 2, 257
     ring = KvRing(layers=1, heads=H, streams=1, capacity=C, dtype=dtype, wrap=True, max_position=1024)
     held = Held(ring)
     fill(ring, 0, 0, 400, 5)
@@ -161,10 +163,11 @@ def test_chain_is_append_attend_in_sequence(dtype, C, start, T):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
-def test_what_is_masked_does_not_matter(dtype, bad):
+@pytest.mark.parametrize("T", [7, 13, 20, 50])
+def test_what_is_masked_does_not_matter(dtype, bad, T):
     """NaN and infinities in empty slots, in slots of positions the query may not see (later ones, and expired
     ones that another node still sees), in absent nodes and in nodes off the path."""
-    H, C, T, base = 2, 90, 20, 150
+    H, C, base = 2, 90, 150
     ring = KvRing(layers=1, heads=H, streams=1, capacity=C, dtype=dtype, wrap=True, max_position=1024)
     held = Held(ring)
     fill(ring, 0, 0, base, 3)
@@ -175,12 +178,12 @@ def test_what_is_masked_does_not_matter(dtype, bad):
     sp[5], sp[40] = base, base + 3     # left over from a longer run: not below the base
     for j in (0, 17, 33, 89, 5, 40):
         kv[:, :, j] = bad
-    # 0 - 1 - 2 - 3 a chain, 4.. hang on the ring; node 8 absent, node 9 off every other path
+    # 0 - 1 - 2 - 3 a chain, 4.. hang on the ring; node 4 absent, node 5 (and the last) off every other path
     tree = [-1, 0, 1, 2] + [-1] * (T - 4)
-    tree[8] = -2
+    tree[4] = -2
     qkv = normal((1, T, 3 * H * HD), 4)
-    qkv[0, 8] = bad
-    qkv[0, 9] = bad
+    for t in (4, 5, T - 1):
+        qkv[0, t] = bad
     # the slot of position base - C + 1 is seen at depth 0, expired for depth >= 1
     edge = (base - C + 1) % C
     kv[1, :, edge] = bad
@@ -192,7 +195,7 @@ def test_what_is_masked_does_not_matter(dtype, bad):
     for t in (1, 2, 3):  # depth >= 1: nothing bad is visible
         assert np.isfinite(got[t]).all(), t
         assert (np.abs(got[t] - want[t]) <= bound[t]).all(), t
-    # without the bad value at the edge the siblings are clean too, whatever node 9 holds
+    # without the bad value at the edge the siblings are clean too, whatever nodes 5 and T - 1 hold
     kv[1, :, edge] = 0.5
     out = ring.tree_attend(0, [0], [base], [tree], qkv)
     ring.sync()
@@ -200,7 +203,7 @@ def test_what_is_masked_does_not_matter(dtype, bad):
     k, v, s = held.item(0, 0)
     want, bound = attend_tree(k, v, s, base, tree, qkv[0].cpu().numpy(), dtype, H)
     for t in range(T):
-        if t in (8, 9):
+        if t in (4, 5, T - 1):
             continue
         assert np.isfinite(got[t]).all(), t
         assert (np.abs(got[t] - want[t]) <= bound[t]).all(), t
@@ -267,9 +270,9 @@ def test_rejected_and_absent_items_leave_their_rows():
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("C,wrap,T", [(20, True, 33), (200, True, 64), (400, False, 9)])
-def test_commit_is_rope_append_along_the_path(dtype, C, wrap, T):
-    L, H, n = 3, 5, 4
+@pytest.mark.parametrize("C,wrap,T,H", [(20, True, 33, 5), (200, True, 64, 1), (400, False, 9, 12), (100, True, 64, 64)])
+def test_commit_is_rope_append_along_the_path(dtype, C, wrap, T, H):
+    L, n = 3, 4
     bases = [0, 7, C - T - 1 if not wrap else C - 3, 2 * C + 5 if wrap else 3]
     a = KvRing(layers=L, heads=H, streams=6, capacity=C, dtype=dtype, wrap=wrap, max_position=1024)
     b = KvRing(layers=L, heads=H, streams=6, capacity=C, dtype=dtype, wrap=wrap, max_position=1024)
@@ -376,6 +379,54 @@ def test_bounded_wait_runs_out_and_the_context_recovers():
     ring.set_wait_limit(0)
     assert torch.equal(ring.tree_attend(0, [0, 1], [200, 200], trees, qkv), want)
     ring.sync()
+
+
+@pytest.mark.parametrize("H", [1, 64])
+def test_head_counts(H):
+    """The fewest and the most heads."""
+    C, T = 70, 21
+    ring = KvRing(layers=1, heads=H, streams=2, capacity=C, dtype="bf16", wrap=True, max_position=512)
+    for s in range(2):
+        fill(ring, 0, s, 60 + 30 * s, s)
+    trees = [tree_of("random", T, i) for i in range(2)]
+    qkv = normal((2, T, 3 * H * HD), 3)
+    out = ring.tree_attend(0, [0, 1], [60, 90], trees, qkv)
+    ring.sync()
+    check(ring, 0, [0, 1], [60, 90], trees, qkv, out)
+
+
+def test_first_calls_may_be_captured():
+    """Nothing has to run before a capture: the first call of every operator of a process, in a graph."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from mockbird_b200 import KvRing, beam_select
+H, T, n = 2, 5, 2
+ring = KvRing(layers=2, heads=H, streams=n, capacity=40, dtype="f16", wrap=True, max_position=128)
+ids = torch.arange(n, dtype=torch.int32, device="cuda")
+pos = torch.zeros(n, dtype=torch.int32, device="cuda")
+tree = torch.tensor([[-1, 0, 1, 1, -1]] * n, dtype=torch.int32, device="cuda")
+leaf = torch.tensor([2, 4], dtype=torch.int32, device="cuda")
+qkv = torch.randn(2, n, T, 3 * H * 64, device="cuda")
+x, s = torch.randn(1, n, 5000, device="cuda"), torch.zeros(1, n, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = ring.tree_attend(0, ids, pos, tree, qkv[0])
+    nxt = ring.tree_commit(0, ids, pos, tree, leaf, qkv)
+    parents, tokens, scores, _ = beam_select(x, s)
+    ring.reorder(ids.view(1, n), parents)
+g.replay()
+ring.sync()
+assert nxt.tolist() == [3, 1] and torch.isfinite(out).all() and torch.isfinite(scores).all(), (nxt, scores)
+want = beam_select(x, s)
+assert torch.equal(want[0], parents) and torch.equal(want[1], tokens) and torch.equal(want[2], scores)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("n,T,dtype", [(40, 16, "bf16"), (130, 5, "f32"), (70, 20, "f16")])
