@@ -165,14 +165,38 @@ __device__ __forceinline__ void fetch_batch(const T* row, const Segment<T>& sg, 
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
+// The words of the row's seen mask that a lane's batch needs: a vector's codes lie in two of them at most.
+template <typename T, bool SEEN>
+__device__ __forceinline__ void batch_masks(const Row<T, SEEN>& row, const Segment<T>& sg, int q, int l,
+                                            uint32_t (&w)[Segment<T>::VECS][2]) {
+    if constexpr (SEEN) {
+        constexpr int E = Segment<T>::E;
+#pragma unroll
+        for (int v = 0; v < Segment<T>::VECS; v++) {
+            const bool in = l + 32 * (q * Segment<T>::VECS + v) < sg.nvec;
+            const int j = sg.code(q, l, v * E);
+            w[v][0] = in ? row.seen[j >> 5] : 0u;
+            w[v][1] = in ? row.seen[(j + E - 1) >> 5] : 0u;
+        }
+    }
+}
+
 // the batch's values, -inf behind the segment's last vector
 template <typename T, bool SEEN>
 __device__ __forceinline__ void batch_values(const Row<T, SEEN>& row, const Segment<T>& sg, int q, int l,
-                                             const uint4* raw, float (&x)[16]) {
+                                             const uint4* raw, const uint32_t (&w)[Segment<T>::VECS][2],
+                                             float (&x)[16]) {
+    constexpr int E = Segment<T>::E;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-        const bool in = l + 32 * (q * Segment<T>::VECS + e / Segment<T>::E) < sg.nvec;
-        x[e] = in ? row.one(reinterpret_cast<const T*>(raw)[e], sg.code(q, l, e)) : -INFINITY;
+        const bool in = l + 32 * (q * Segment<T>::VECS + e / E) < sg.nvec;
+        const int j = sg.code(q, l, e), j0 = sg.code(q, l, e / E * E);
+        float v = to_f(reinterpret_cast<const T*>(raw)[e]);
+        if constexpr (SEEN) {
+            const uint32_t word = (j >> 5) == (j0 >> 5) ? w[e / E][0] : w[e / E][1];
+            v = penalised(v, (word >> (j & 31)) & 1u, row.penalty);
+        }
+        x[e] = in ? v : -INFINITY;
     }
 }
 
@@ -251,12 +275,14 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, 2) beam_select_kernel(BeamArg
 #pragma unroll
         for (int i = 0; i < BEAM_STAGES; i++) fetch_batch(row.p, sg, i, lane, stage + i * 128);
         for (int q = 0, st = 0, in_cell = 0; q < nb; q++) {
+            uint32_t masks[VECS][2];
+            batch_masks(row, sg, q, lane, masks);
             asm volatile("cp.async.wait_group %0;" ::"n"(BEAM_STAGES - 1) : "memory");
             uint4 raw[VECS];
 #pragma unroll
             for (int v = 0; v < VECS; v++) raw[v] = stage[st * 128 + v * 32 + lane];
             float x[16];
-            batch_values(row, sg, q, lane, raw, x);
+            batch_values(row, sg, q, lane, raw, masks, x);
             fetch_batch(row.p, sg, q + BEAM_STAGES, lane, stage + st * 128);
             st = st + 1 == BEAM_STAGES ? 0 : st + 1;
             const float m = tree_max(x);
@@ -338,40 +364,40 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, 2) beam_select_kernel(BeamArg
             pooled += __popc(in);
         };
         if (sg.head | sg.tail) add_to_pool(edge, sg.edge(lane), edge > -INFINITY);
-        // The cells that reach `need`, 32 at a time, one to a lane.
+        // The batches of the lanes' cells that reach `need`, 32 at a time, one to a lane.
         const int used = nb ? (nb - 1) / cell + 1 : 0;
-        int mine = -1, taken = 0;  // this lane's: cell * 32 + its lane
+        int mine_q = nb, mine_l = 0, taken = 0;  // this lane's batch (nb: none) and whose it is
         auto flush = [&] {
-            for (int g = 0; g < cell; g++) {
-                const int q = mine < 0 ? nb : min((mine >> 5) * cell + g, nb), l = mine & 31;  // nb: nothing
-                uint4 raw[VECS];
+            uint4 raw[VECS];
+            uint32_t masks[VECS][2];
 #pragma unroll
-                for (int v = 0; v < VECS; v++) {
-                    const int at = l + 32 * (q * VECS + v);
-                    if (at < sg.nvec) raw[v] = reinterpret_cast<const uint4*>(row.p + sg.body)[at];
-                }
-                float x[16];
-                batch_values(row, sg, q, l, raw, x);
-                unsigned in = 0u;  // the lane's values that reach `need`, taken one by one through shared memory
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    xs[e * 32 + lane] = x[e];
-                    in |= x[e] >= need ? 1u << e : 0u;
-                }
-                while (__any_sync(ALL, in != 0u)) {
-                    const int e = in ? __ffs(in) - 1 : 0;
-                    add_to_pool(xs[e * 32 + lane], sg.code(q, l, e), in != 0u);
-                    in &= in - 1u;
-                }
+            for (int v = 0; v < VECS; v++) {
+                const int at = mine_l + 32 * (mine_q * VECS + v);
+                if (at < sg.nvec) raw[v] = reinterpret_cast<const uint4*>(row.p + sg.body)[at];
             }
-            mine = -1, taken = 0;
+            batch_masks(row, sg, mine_q, mine_l, masks);
+            float x[16];
+            batch_values(row, sg, mine_q, mine_l, raw, masks, x);
+            unsigned in = 0u;  // the lane's values that reach `need`, taken one by one through shared memory
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                xs[e * 32 + lane] = x[e];
+                in |= x[e] >= need ? 1u << e : 0u;
+            }
+            while (__any_sync(ALL, in != 0u)) {
+                const int e = in ? __ffs(in) - 1 : 0;
+                add_to_pool(xs[e * 32 + lane], sg.code(mine_q, mine_l, e), in != 0u);
+                in &= in - 1u;
+            }
+            mine_q = nb, taken = 0;
         };
         for (int k = 0; k < used; k++) {
             const float c = __bfloat162float(sm.cell[warp][k][lane]);
-            for (unsigned in = __ballot_sync(ALL, c >= need && c > -INFINITY); in; in &= in - 1u) {
-                if (lane == taken) mine = k * 32 + __ffs(in) - 1;
-                if (++taken == 32) flush();
-            }
+            for (unsigned in = __ballot_sync(ALL, c >= need && c > -INFINITY); in; in &= in - 1u)
+                for (int q = k * cell; q < min((k + 1) * cell, nb); q++) {
+                    if (lane == taken) mine_q = q, mine_l = __ffs(in) - 1;
+                    if (++taken == 32) flush();
+                }
         }
         if (taken) flush();
         cut();
@@ -447,14 +473,13 @@ __global__ void __launch_bounds__(32 * BEAM_WARPS, 2) beam_select_kernel(BeamArg
         }
         if (tid < B) sm.pick[tid] = INT_MAX;
         __syncthreads();
-        if (tid < units) {
-            const double bound = (double)sm.bound - NEAR;
-            for (int k = 0; v > -INFINITY && v >= bound;) {
-                const int r = tid / segs;
-                sm.cand[atomicAdd(&sm.count, 1)] = Candidate{order_key(v), r * V + at, r};
-                if (++k == B) break;
-                v = value(tid, k, at);
-            }
+        const double bound = (double)sm.bound - NEAR;
+        for (int i = tid; i < units * B; i += 32 * BEAM_WARPS) {
+            const int u = i / B;
+            if (sm.head[u] < sm.bound - 2.f * (float)NEAR - fabsf(sm.bound) * 1e-6f) continue;  // (rounded down)
+            v = value(u, i % B, at);
+            if (v > -INFINITY && v >= bound)
+                sm.cand[atomicAdd(&sm.count, 1)] = Candidate{order_key(v), u / segs * V + at, u / segs};
         }
         __syncthreads();
         const int n = sm.count;
