@@ -62,12 +62,15 @@ def _ptr(t) -> ctypes.c_void_p:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _used_on(stream, t: torch.Tensor) -> None:
-    """Tell the caching allocator that `t`, made on the current stream, is used on
-    `stream`: its memory is then not handed out again before that use is over."""
-    if stream is not None and t.is_cuda:
-        t.record_stream(stream if isinstance(stream, torch.cuda.Stream)
-                        else torch.cuda.ExternalStream(int(stream), device=t.device))
+def _made_on(stream, device, make):
+    """make(), with what it allocates and copies ordered on `stream` (None: the current one): memory of the
+    current stream's pool may still be in use by work queued there, which a call on `stream` does not wait for."""
+    if stream is None:
+        return make()
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    with torch.cuda.stream(stream):
+        return make()
 
 
 _TORCH_DTYPE = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
@@ -278,8 +281,8 @@ class KvRing:
         s, p = self._id_array("streams", streams, (n,), stream), self._id_array("positions", positions, (n,), stream)
         tree = self._id_array("parents", parents, (n, nodes), stream)
         if out is None:
-            out = torch.empty(n, nodes, self.hidden, dtype=torch.float32, device=self.device)
-            _used_on(stream, out)
+            out = _made_on(stream, self.device, lambda: torch.empty(n, nodes, self.hidden, dtype=torch.float32,
+                                                                    device=self.device))
         else:
             self._array("out", out, (n, nodes, self.hidden), torch.float32)
         self._check(self.lib.mb_tree_attend(self.ctx, layer, n, nodes, s.data_ptr(), p.data_ptr(), tree.data_ptr(),
@@ -297,8 +300,8 @@ class KvRing:
         s, p = self._id_array("streams", streams, (n,), stream), self._id_array("positions", positions, (n,), stream)
         tree, leaf = self._id_array("parents", parents, (n, nodes), stream), self._id_array("leaves", leaves, (n,), stream)
         if next_positions is None:
-            next_positions = torch.empty(n, dtype=torch.int32, device=self.device)
-            _used_on(stream, next_positions)
+            next_positions = _made_on(stream, self.device,
+                                      lambda: torch.empty(n, dtype=torch.int32, device=self.device))
         else:
             self._array("next_positions", next_positions, (n,), torch.int32)
         self._check(self.lib.mb_tree_commit(self.ctx, layer, qkv.shape[0], n, nodes, s.data_ptr(), p.data_ptr(),
@@ -330,11 +333,10 @@ class KvRing:
         """An int32 array of `shape`: a device tensor as it is, or host values copied to the device."""
         if isinstance(values, torch.Tensor) and values.is_cuda:
             return self._array(name, values, shape, torch.int32)
-        t = torch.as_tensor(np.ascontiguousarray(values, np.int32), device=self.device)
-        if shape is not None and t.shape != shape:
-            raise ValueError(f"{name} must be of shape {list(shape)} (got {list(t.shape)})")
-        _used_on(stream, t)
-        return t
+        a = np.ascontiguousarray(values, np.int32)
+        if shape is not None and a.shape != shape:
+            raise ValueError(f"{name} must be of shape {list(shape)} (got {list(a.shape)})")
+        return _made_on(stream, self.device, lambda: torch.as_tensor(a, device=self.device))
 
     def _tree_shape(self, qkv, dims: int) -> tuple[int, int]:
         """(items, nodes) of a tree's qkv rows, [..][n][nodes][3*H*64]."""
@@ -600,15 +602,17 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
         raise TypeError("logits' rows must be contiguous and evenly spaced")
     dev, shape = logits.device, (groups, beams)
     _beam_array("scores", scores, torch.float32, shape, dev)
-    new = torch.empty((3 if finished is None else 4, groups, beams), dtype=torch.int32, device=dev)
-    _used_on(stream, new)
-    parents, tokens, out, *done = new.unbind()
-    out = out.view(torch.float32)
-    done = done[0] if done else None
+
+    def outputs():
+        parents = torch.empty_like(scores, dtype=torch.int32)
+        done = None if finished is None else torch.empty_like(parents)
+        return parents, torch.empty_like(parents), torch.empty_like(scores), done
+
     if finished is not None:
         _beam_array("finished", finished, torch.int32, shape, dev)
     if seen is not None:
         _beam_array("seen", seen, torch.int32, (groups, beams, codes // 32), dev)
+    parents, tokens, out, done = _made_on(stream, dev, outputs)
     if stream is None:
         stream = _raw_stream(dev.index) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
     elif isinstance(stream, torch.cuda.Stream):

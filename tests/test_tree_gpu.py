@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from mockbird_b200 import KvRing, MockbirdError
+from mockbird_b200 import KvRing, MockbirdError, beam_select
 from search_util import HD, TORCH_DT, attend_tree, path_to
 
 pytestmark = pytest.mark.gpu
@@ -359,6 +359,30 @@ def test_capture_streams_and_determinism():
     torch.cuda.synchronize()
     ring.sync()
     assert all(torch.equal(x, wa) and torch.equal(y, wb) for x, y in got)
+
+
+def test_outputs_of_another_stream_are_not_memory_in_use():
+    """A call on another stream does not get memory that work queued on the current stream still uses."""
+    H, C, T = 4, 64, 8
+    ring = KvRing(layers=1, heads=H, streams=1, capacity=C, dtype="f32", wrap=True, max_position=256)
+    fill(ring, 0, 0, 50, 1)
+    trees, qkv = [tree_of("chain", T)], normal((1, T, 3 * H * HD), 2)
+    x, s = normal((1, 4, 1000), 3), torch.zeros(1, 4, device=DEV)
+    want, chosen = ring.tree_attend(0, [0], [50], trees, qkv), beam_select(x, s)
+    ring.sync()
+    other = torch.cuda.Stream()
+    torch.cuda._sleep(200_000_000)
+    held = [torch.empty(1, T, H * HD, device=DEV).fill_(3.0) for _ in range(4)]
+    held += [torch.empty(1, 4, dtype=torch.int32, device=DEV).fill_(3) for _ in range(8)]
+    busy = {t.data_ptr() for t in held}
+    del held
+    got = ring.tree_attend(0, [0], [50], trees, qkv, stream=other)
+    picked = beam_select(x, s, stream=other.cuda_stream)
+    assert not busy & {t.data_ptr() for t in (got, *picked[:3])}
+    other.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(picked[:3], chosen[:3]))
+    ring.sync()
 
 
 def test_bounded_wait_runs_out_and_the_context_recovers():
