@@ -144,7 +144,7 @@ __device__ __forceinline__ void pair_parts(float x, float y, uint32_t* p) {
 // own stage, and it keeps the running maximum, sum and context of its rows in
 // registers, so nothing in the loop waits for another warp; while one warp's tile
 // is on its way the SM's other warps compute (16 of them, 20 with PACK, 12 with two
-// matrix tiles of rows).  The tree's own K and V come first, as tiles of the same
+// matrix tiles of rows, MT = 2).  The tree's own K and V come first, as tiles of the same
 // layout, built from the qkv rows.  At the end the warps join through shared
 // memory, then the blocks of the cluster through distributed shared memory: no
 // scratch in device memory, so calls share nothing.
@@ -153,8 +153,12 @@ __device__ __forceinline__ void pair_parts(float x, float y, uint32_t* p) {
 // the same 8 nodes, whose products the lane that holds both adds up.
 //
 // mma.sync and not tcgen05: with 5 to 16 query rows per K and V row the 128 rows of
-// a tcgen05 tile would be almost empty.  The tensor pipe is 45 % busy where HBM
-// limits (16 nodes, bf16), and what limits 64 nodes.
+// a tcgen05 tile would be almost empty.  Measured (12 heads, the live window's bytes
+// over the time): 64 streams of 5 nodes over 512-slot fp32 rings 39 us, 4.6 TB/s, the
+// tensor pipe 32 % busy; 64 of up to 16 nodes over ragged bf16 rings of up to 4096
+// slots 99 us, 5.4 TB/s, 54 %: HBM limits the loop (89 us with the arithmetic left
+// out), the blocks' start and join the rest.  16 of 64 nodes over 2048-slot f16 rings
+// 50 us: the products' four parts and, for the longest windows, their latency.
 constexpr int WARPS = 4, SORT_MAX = 256, SMS = 148;
 
 template <typename T>
@@ -188,8 +192,9 @@ struct alignas(1024) TreeSmem {
     int item;                                                // the block's (sort)
 };
 
-template <typename T, int MT, bool PACK>
-__global__ void __launch_bounds__(32 * WARPS, MT == 2 ? (sizeof(T) == 4 ? 2 : 3) : PACK ? 5 : 4)
+// CAP: the most nodes of a tree
+template <typename T, int MT, bool PACK, int CAP>
+__global__ void __launch_bounds__(32 * WARPS, MT == 2 ? 3 : PACK ? 5 : 4)
     tree_attend_kernel(const __grid_constant__ CUtensorMap map, RingView r, int n, int nodes, int qtiles, int splits,
                        bool sort, const int32_t* __restrict__ streams, const int32_t* __restrict__ positions,
                        const int32_t* __restrict__ parents, const float* __restrict__ qkv, float* __restrict__ out) {
@@ -231,7 +236,7 @@ __global__ void __launch_bounds__(32 * WARPS, MT == 2 ? (sizeof(T) == 4 ? 2 : 3)
     // (in the order the matrix instructions take them: pair i of a fragment is row grp (i even) or grp + 8, then,
     // 16-bit, the pair of dims 8 further on), the tree's K and V, the ring's first tiles.
     constexpr int FRAGS = MT * QSTEPS / WARPS, PAIRS = F32 ? 1 : 2;  // pairs of a row
-    constexpr int TREE = ((MT == 1 ? NODES : TREE_MAX_NODES) + TS - 1) / TS, RB = TS / WARPS;  // tree tiles; a warp's rows
+    constexpr int TREE = (CAP + TS - 1) / TS, RB = TS / WARPS;  // tree tiles; a warp's rows
     const int t0 = qt * NODES;
     const size_t row_f = (size_t)3 * H * HD;
     const float* rows = qkv + (size_t)item * nodes * row_f + h * HD;
@@ -942,12 +947,12 @@ bool make_ring_map(CUtensorMap* m, const RingView& r) {
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int MT, bool PACK>
+template <typename T, int MT, bool PACK, int CAP>
 cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* streams, const int32_t* positions,
                       const int32_t* parents, const float* qkv, float* out, cudaStream_t st) {
     using Sm = TreeSmem<T, MT, PACK>;
     constexpr int smem = sizeof(Sm);
-    const auto kernel = tree_attend_kernel<T, MT, PACK>;
+    const auto kernel = tree_attend_kernel<T, MT, PACK, CAP>;
     // the opt-in to more than 48 KB of shared memory, once per device
     static std::atomic<uint64_t> opted{0};
     int dev = 0;
@@ -964,8 +969,11 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
     const int qtiles = (nodes + Sm::NODES - 1) / Sm::NODES;
     const int tiles = (r.capacity + Tile<T>::SLOTS - 1) / Tile<T>::SLOTS + (nodes + Tile<T>::SLOTS - 1) / Tile<T>::SLOTS;
     const int blocks = n * r.heads * qtiles;
+    // splits: single calls of few blocks need them (one stream of 4000 slots 12.6 us, 39 without; 4 of 1000 slots
+    // 18.7, 25.4 without); past two blocks per SM a block's start costs more than it saves (384 blocks: 53 us, 57 as 768)
     int splits = 1;
     while (splits < 8 && blocks * splits < 2 * SMS && splits * WARPS < tiles) splits *= 2;
+    // longest first: 99.5 us for ragged windows (118.7 in the given order); 2 % lost where all are alike
     const bool sort = n > 1 && n <= SORT_MAX && blocks * splits > 2 * SMS;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(blocks * splits);
@@ -985,9 +993,19 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
 template <typename T>
 cudaError_t attend_t(const RingView& r, int n, int nodes, const int32_t* streams, const int32_t* positions,
                      const int32_t* parents, const float* qkv, float* out, cudaStream_t st) {
-    if (nodes <= 8) return attend_mt<T, 1, true>(r, n, nodes, streams, positions, parents, qkv, out, st);
-    if (nodes <= 16) return attend_mt<T, 1, false>(r, n, nodes, streams, positions, parents, qkv, out, st);
-    return attend_mt<T, 2, false>(r, n, nodes, streams, positions, parents, qkv, out, st);
+    // At most 8 nodes, two parts to a matrix tile: 64 streams of 5 nodes 39 us (50 as rows of 16; C = 512, fp32),
+    // 55 us (59; C = 1024, bf16).
+    if (nodes <= 8) return attend_mt<T, 1, true, 8>(r, n, nodes, streams, positions, parents, qkv, out, st);
+    // 9 to 16: one tile of rows per warp (60 us for 64 streams of 12 nodes, C = 1024, bf16; 83 as two, half empty).
+    if (nodes <= 16) return attend_mt<T, 1, false, 16>(r, n, nodes, streams, positions, parents, qkv, out, st);
+    // More: blocks of 16 nodes each, which read K and V again, from L2, but start and run with more warps per SM --
+    // 48 nodes 129 us (157 as blocks of 32; bf16) and 218 (301; fp32), 24 nodes 150 (164; fp32).  Only 16-bit rings
+    // with up to 32 nodes and blocks enough do better with two tiles of rows per warp: 85 us (88), but 18.8 (16.7) at
+    // 4 streams.
+    if constexpr (sizeof(T) == 2)
+        if (nodes <= 32 && n * r.heads >= 2 * SMS)
+            return attend_mt<T, 2, false, 32>(r, n, nodes, streams, positions, parents, qkv, out, st);
+    return attend_mt<T, 1, false, TREE_MAX_NODES>(r, n, nodes, streams, positions, parents, qkv, out, st);
 }
 
 template <typename T>

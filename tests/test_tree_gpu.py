@@ -163,12 +163,12 @@ def test_chain_is_append_attend_in_sequence(dtype, C, start, T):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
-@pytest.mark.parametrize("T", [7, 13, 20, 50])
-def test_what_is_masked_does_not_matter(dtype, bad, T):
+@pytest.mark.parametrize("T,H,n", [(7, 2, 1), (13, 2, 1), (20, 2, 1), (50, 2, 1), (20, 64, 5)])
+def test_what_is_masked_does_not_matter(dtype, bad, T, H, n):
     """NaN and infinities in empty slots, in slots of positions the query may not see (later ones, and expired
     ones that another node still sees), in absent nodes and in nodes off the path."""
-    H, C, base = 2, 90, 150
-    ring = KvRing(layers=1, heads=H, streams=1, capacity=C, dtype=dtype, wrap=True, max_position=1024)
+    C, base = 90, 150
+    ring = KvRing(layers=1, heads=H, streams=1, capacity=C, dtype=dtype, wrap=True, max_position=1024, max_batch=n)
     held = Held(ring)
     fill(ring, 0, 0, base, 3)
     sp = held.slot_pos[0, 0]
@@ -187,8 +187,12 @@ def test_what_is_masked_does_not_matter(dtype, bad, T):
     # the slot of position base - C + 1 is seen at depth 0, expired for depth >= 1
     edge = (base - C + 1) % C
     kv[1, :, edge] = bad
-    out = ring.tree_attend(0, [0], [base], [tree], qkv)
+    # (n equal items: from 296 heads in all on, 16-bit rings take two tiles of rows per warp)
+    many = qkv.expand(n, -1, -1).contiguous()
+    out = ring.tree_attend(0, [0] * n, [base] * n, [tree] * n, many, out=torch.zeros(n, T, H * HD, device=DEV))
     ring.sync()
+    for i in range(1, n):
+        assert torch.equal(out[i].nan_to_num(7.0), out[0].nan_to_num(7.0))
     got = out[0].double().cpu().numpy()
     k, v, s = held.item(0, 0)
     want, bound = attend_tree(k, v, s, base, tree, qkv[0].cpu().numpy(), dtype, H)
@@ -197,7 +201,7 @@ def test_what_is_masked_does_not_matter(dtype, bad, T):
         assert (np.abs(got[t] - want[t]) <= bound[t]).all(), t
     # without the bad value at the edge the siblings are clean too, whatever nodes 5 and T - 1 hold
     kv[1, :, edge] = 0.5
-    out = ring.tree_attend(0, [0], [base], [tree], qkv)
+    out = ring.tree_attend(0, [0] * n, [base] * n, [tree] * n, many)
     ring.sync()
     got = out[0].double().cpu().numpy()
     k, v, s = held.item(0, 0)
@@ -453,7 +457,8 @@ assert torch.equal(want[0], parents) and torch.equal(want[1], tokens) and torch.
     assert r.returncode == 0, r.stderr[-2000:]
 
 
-@pytest.mark.parametrize("n,T,dtype", [(40, 16, "bf16"), (130, 5, "f32"), (70, 20, "f16")])
+@pytest.mark.parametrize("n,T,dtype", [(40, 16, "bf16"), (130, 5, "f32"), (70, 20, "f16"), (70, 31, "bf16"),
+                                       (60, 32, "f32"), (50, 64, "bf16")])
 def test_many_ragged_items(n, T, dtype):
     """More blocks than run at once (their items are then taken longest window first), equal windows and empty
     ones among them; every row against a call of its own."""
