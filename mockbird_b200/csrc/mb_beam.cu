@@ -84,6 +84,10 @@ __device__ __forceinline__ double key_value(unsigned long long key) {
 // the group's sums are taken again in fp64, by the same warps, and the merge
 // repeated, so the order is always that of the values in 64 bits.  (All sums in fp64 would cost 14 fp64 operations per logit:
 // 1.4e12 logits/s on this part's fp64 units, against the 1.6e12 fp32 logits/s of HBM.)
+//
+// Measured: 44 us for 16 groups of 16 x 131071 fp32 logits, 134 MB, of which the pass
+// is 22 us at 6.2 TB/s; 23 us for 32 groups of 8 x 50021 bf16 logits, the pass bound by
+// exponentials and conversions; a group of 4 x 1024 6 us, a chain of waits.
 constexpr int BEAM_WARPS = 16, BEAM_CLUSTER = 8, UNITS = BEAM_WARPS * BEAM_CLUSTER;
 constexpr int CELLS = 16, BEAM_STAGES = 2, POOL = 64;  // per warp (and lane)
 constexpr double NEAR = 8e-6;
