@@ -202,7 +202,7 @@ MB_API int mb_ring_write(mb_ctx* ctx, int32_t layer, int32_t stream, int32_t fir
  * them), with K after RoPE and V rounded to the storage type -- what
  * mb_append_attend gives for t when the nodes of its path are appended one after
  * another.  qkv: device f32 [n][nodes][3*heads*64] (read-only); out: device f32
- * [n][nodes][heads*64], rows of absent nodes and of rejected items left as they
+ * [n][nodes][heads*64], apart from qkv, rows of absent nodes and of rejected items left as they
  * were.  Live K and V must be finite for finite results; what dead slots and
  * nodes off the path hold does not matter.  A stream may appear in several items
  * (the rings are only read). */
@@ -234,7 +234,7 @@ MB_API int mb_sync(mb_ctx* ctx, void* cuda_stream);
 
 /* Failure detection.  No counterpart in the reference, whose WebGPU queue has no
  * timeouts (its warm-up checks, gpu.ts:201-234, only catch wrong results).  The
- * decode kernels of this context wait for their K/V chunks at most `cycles` SM
+ * decode and tree attention kernels of this context wait for their K/V chunks at most `cycles` SM
  * clock cycles (0 restores the default, about 2 s); a wait that runs out skips
  * the chunk, lets its copies land (at the default bound), and the next mb_sync
  * reports MB_ERR_TIMEOUT.  A negative value is the test of that path: the waits

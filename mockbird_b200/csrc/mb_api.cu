@@ -588,6 +588,9 @@ MB_API int mb_tree_attend(mb_ctx* c, int32_t layer, int32_t n, int32_t nodes, co
     if (!streams || !positions || !parents || !qkv || !out || !aligned(qkv, 16) || !aligned(out, 16) ||
         !aligned(streams, 4) || !aligned(positions, 4) || !aligned(parents, 4))
         return fail(c, MB_ERR_ARG, "null or misaligned device pointer");
+    // (a block reads the rows of one head of an item while another writes the item's context)
+    const size_t rows = (size_t)n * nodes * c->cfg.heads * HD;
+    if (out < qkv + 3 * rows && qkv < out + rows) return fail(c, MB_ERR_ARG, "out overlaps qkv");
     DeviceGuard g(c->cfg.device);
     CK(launch_tree_attend(c->cfg.dtype, ring_view(c, layer), n, nodes, streams, positions, parents, qkv, out,
                           static_cast<cudaStream_t>(cuda_stream)),

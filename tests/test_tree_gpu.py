@@ -524,6 +524,8 @@ def test_refusals():
     refused(TypeError, "streams", streams=torch.zeros(2, dtype=torch.int64, device=DEV))
     refused(ValueError, "out", out=torch.zeros(2, T, H * HD + 1, device=DEV))
     refused(TypeError, "out", out=torch.zeros(2, T, H * HD, dtype=torch.float64, device=DEV))
+    refused(MockbirdError, "out overlaps", out=q.view(-1)[:2 * T * H * HD].view(2, T, H * HD))
+    refused(MockbirdError, "out overlaps", out=q.view(-1)[-2 * T * H * HD:].view(2, T, H * HD))
     many = normal((4, T, 3 * H * HD), 0)
     refused(MockbirdError, "max_batch", streams=[0, 1, 2, 0], positions=[0] * 4, parents=[tree[0]] * 4, qkv=many)
     wide = normal((1, 65, 3 * H * HD), 0)
