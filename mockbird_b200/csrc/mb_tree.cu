@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(32 * WARPS, MT == 2 ? 3 : PACK ? 5 : 4)
     // 16-bit, the pair of dims 8 further on), the tree's K and V, the ring's first tiles.
     constexpr int FRAGS = MT * QSTEPS / WARPS, PAIRS = F32 ? 1 : 2;  // pairs of a row
     constexpr int TREE = (CAP + TS - 1) / TS, RB = TS / WARPS;  // tree tiles; a warp's rows
-    const int t0 = qt * NODES;
+    const int t0 = qt * NODES, last = min(nodes, t0 + NODES);  // no path of this block's nodes has a node behind `last`
     const size_t row_f = (size_t)3 * H * HD;
     const float* rows = qkv + (size_t)item * nodes * row_f + h * HD;
     const int2 parent = tree_parents(parents + (size_t)item * nodes, warp == 0 ? nodes : 0, lane);
@@ -254,17 +254,19 @@ __global__ void __launch_bounds__(32 * WARPS, MT == 2 ? 3 : PACK ? 5 : 4)
         }
     if (rank == 0)
 #pragma unroll
-        for (int u = 0; u < TREE; u++)
+        for (int u = 0; u < TREE; u++) {
+            if (u * TS >= last) break;
 #pragma unroll
             for (int j = 0; j < RB; j++) {
                 const int t = u * TS + warp * RB + j;
-                const float* src = rows + (t < nodes ? t : 0) * row_f;
+                const float* src = rows + (t < last ? t : 0) * row_f;
                 k0[u][j] = reinterpret_cast<const float2*>(src + (size_t)H * HD)[lane];
                 v0[u][j] = reinterpret_cast<const float2*>(src + (size_t)2 * H * HD)[lane];
             }
+        }
     const bool in_range = s >= 0 && s < r.streams && base >= 0;
     const int window = in_range ? min(base, C) : 0;
-    const int ring_tiles = (window + TS - 1) / TS, tree_tiles = (nodes + TS - 1) / TS;
+    const int ring_tiles = (window + TS - 1) / TS, tree_tiles = (last + TS - 1) / TS;
     const int step = splits * WARPS;
     // Warp w of the cluster takes tiles w, w + step, ..: the tree's (at most WARPS: the first tiles of the first
     // block's warps), then the ring's
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(32 * WARPS, MT == 2 ? 3 : PACK ? 5 : 4)
         // rope's factors, q's and K's loads together; absent nodes take the base's
         float2 cs[FRAGS][RH * PAIRS], kcs[TREE][RB];
         auto pos = [&](int t) {
-            const unsigned long long path = t < nodes ? sh.path[t] : 0ull;
+            const unsigned long long path = t < last ? sh.path[t] : 0ull;
             return path ? __popcll(path) - 1 : -1;
         };
 #pragma unroll
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(32 * WARPS, MT == 2 ? 3 : PACK ? 5 : 4)
 #pragma unroll
             for (int u = 0; u < TREE; u++)
 #pragma unroll
-                for (int j = 0; j < RB; j++)
+                for (int j = 0; j < RB && u < tree_tiles; j++)
                     kcs[u][j] = r.rope[(size_t)(base + max(pos(u * TS + warp * RB + j), 0)) * 32 + lane];
             // The tree's K and V: lane i has dims (2 i, 2 i + 1).  Absent nodes and the rows behind the last one
             // become zeros: their weight is zero, and V has to be finite.
