@@ -158,7 +158,7 @@ __device__ __forceinline__ void pair_parts(float x, float y, uint32_t* p) {
 // tensor pipe 32 % busy; 64 of up to 16 nodes over ragged bf16 rings of up to 4096
 // slots 99 us, 5.4 TB/s, 54 %: HBM limits the loop (89 us with the arithmetic left
 // out), the blocks' start and join the rest.  16 of 64 nodes over 2048-slot f16 rings
-// 50 us: the products' four parts and, for the longest windows, their latency.
+// 47 us: the products' four parts and, for the longest windows, their latency.
 constexpr int WARPS = 4, SORT_MAX = 256, SMS = 148;
 
 template <typename T>
@@ -975,7 +975,7 @@ cudaError_t attend_mt(const RingView& r, int n, int nodes, const int32_t* stream
     // 18.7, 25.4 without); past two blocks per SM a block's start costs more than it saves (384 blocks: 53 us, 57 as 768)
     int splits = 1;
     while (splits < 8 && blocks * splits < 2 * SMS && splits * WARPS < tiles) splits *= 2;
-    // longest first: 99.5 us for ragged windows (118.7 in the given order); 2 % lost where all are alike
+    // longest first: 99.5 us for ragged windows (118.7 in the given order); 2 % lost where all are alike (3 % more with a test for that)
     const bool sort = n > 1 && n <= SORT_MAX && blocks * splits > 2 * SMS;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(blocks * splits);
@@ -1001,7 +1001,7 @@ cudaError_t attend_t(const RingView& r, int n, int nodes, const int32_t* streams
     // 9 to 16: one tile of rows per warp (60 us for 64 streams of 12 nodes, C = 1024, bf16; 83 as two, half empty).
     if (nodes <= 16) return attend_mt<T, 1, false, 16>(r, n, nodes, streams, positions, parents, qkv, out, st);
     // More: blocks of 16 nodes each, which read K and V again, from L2, but start and run with more warps per SM --
-    // 48 nodes 129 us (157 as blocks of 32; bf16) and 218 (301; fp32), 24 nodes 150 (164; fp32).  Only 16-bit rings
+    // 48 nodes 125 us (157 as blocks of 32; bf16) and 208 (301; fp32), 24 nodes 146 (164; fp32).  Only 16-bit rings
     // with up to 32 nodes and blocks enough do better with two tiles of rows per warp: 85 us (88), but 18.8 (16.7) at
     // 4 streams.
     if constexpr (sizeof(T) == 2)
