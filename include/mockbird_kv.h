@@ -223,7 +223,8 @@ MB_API int mb_tree_commit(mb_ctx* ctx, int32_t layer, int32_t layers, int32_t n,
 /* Permute the rings of `groups` groups of `beams` (1..16) streams, in place and in
  * every layer: stream streams[g][k] takes the live slots and slot positions that
  * stream streams[g][parents[g][k]] had before the call; -1 leaves it as it is.
- * streams, parents: device int32 [groups][beams], a stream at most once per call
+ * streams, parents: device int32 [groups][beams] (groups * beams at most the
+ * context's streams), a stream at most once per call
  * (a repeat within a group is rejected, one across groups races).  What a slot
  * that is empty in the source held in the destination is left there, empty. */
 MB_API int mb_ring_reorder(mb_ctx* ctx, int32_t groups, int32_t beams, const int32_t* streams,
@@ -408,7 +409,7 @@ MB_API int mb_argmax_penalty(int32_t n, int32_t codes, const float* logits, uint
  *   seen      [groups][beams][codes / 32], updated in place, or NULL (penalty is
  *             then not used); codes must be a multiple of 32
  *   parents, tokens   int32 [groups][beams] out
- * 1 <= codes <= 2^24.  Async on cuda_stream. */
+ * 1 <= codes <= 2^24, groups <= 65535, row_stride <= 2^32.  Async on cuda_stream. */
 MB_API int mb_beam_select(int32_t groups, int32_t beams, int32_t codes, int32_t dtype, const void* logits,
                           int64_t row_stride, const float* scores, float* scores_out, const int32_t* finished,
                           int32_t* finished_out, int32_t end_id, uint32_t* seen, float penalty, int32_t* parents,
